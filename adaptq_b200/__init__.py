@@ -9,7 +9,9 @@ NVIDIA B200 (sm_100a), behind upstream's own interfaces:
   model behind one handle);
 * ``adaptq_b200.runtime`` (upstream's second stack: ``RuntimeContext``, AQSS v2
   snapshots, ``IKernelBackend``) and ``adaptq_b200.hf_cache`` (Hugging Face
-  ``DynamicCache`` + fused attention function).
+  ``DynamicCache`` + fused attention function);
+* ``PagedKVCache`` and ``Rotary``: the same rows in pages, for batches whose sequences
+  have different lengths, with positions rotated on the way (include/adaptq_paged.h).
 """
 from ._lib import LIB_PATH, last_error, load  # noqa: F401
 from .core import Engine  # noqa: F401
@@ -23,4 +25,10 @@ def __getattr__(name):
     if name in ("AdaptQAttention", "BatchedAdaptQAttention"):  # lazy: importing torch is slow
         from . import torch_adapter
         return getattr(torch_adapter, name)
+    if name == "PagedKVCache":
+        from . import paged
+        return paged.PagedKVCache
+    if name == "Rotary":
+        from . import rotary
+        return rotary.Rotary
     raise AttributeError(name)

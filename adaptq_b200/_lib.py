@@ -24,6 +24,20 @@ class MhaInfo(C.Structure):
                 ("v_mass", C.c_float), ("device_bytes", C.c_size_t)]
 
 
+class Paged(C.Structure):
+    """adaptq_paged_t"""
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("signs", C.c_void_p), ("status", C.c_void_p), ("n_pages", C.c_int64), ("n_kv_heads", C.c_int),
+                ("page_size", C.c_int), ("dim", C.c_int), ("k_bits", C.c_int), ("v_bits", C.c_int), ("device", C.c_int)]
+
+
+class RotaryDesc(C.Structure):
+    """adaptq_rotary_t"""
+    _fields_ = [("turns", C.c_void_p), ("factor", C.c_float), ("dim", C.c_int), ("interleaved", C.c_int)]
+
+
+_rows = [C.c_void_p, C.c_int64, C.c_int64]  # a tensor and its two outer strides
+
 # name -> (restype, argtypes); every symbol declared in include/*.h
 SYMBOLS = {
     "adaptq_last_error": (C.c_char_p, []),
@@ -91,6 +105,17 @@ SYMBOLS = {
     "adaptq_kernel_kdot_batch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "adaptq_kernel_vaccum_batch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int]),
     "adaptq_kernel_backend_name": (C.c_char_p, []),
+    # include/adaptq_paged.h
+    "adaptq_rotary_apply": (C.c_int, [C.c_void_p, *_rows, *_rows, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int,
+                                      C.c_int, C.c_void_p]),
+    "adaptq_paged_signs": (C.c_int, [C.c_uint64, C.c_int, C.c_int, C.c_void_p]),
+    "adaptq_paged_append": (C.c_int, [C.c_void_p, *_rows, *_rows, C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int,
+                                      C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p]),
+    "adaptq_paged_read": (C.c_int, [C.c_void_p, *_rows, *_rows, C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p,
+                                    C.c_int, C.c_int64, C.c_void_p]),
+    "adaptq_paged_attend_workspace": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "adaptq_paged_attend": (C.c_int, [C.c_void_p, *_rows, *_rows, C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int,
+                                      C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "adaptq_inject_failure": (C.c_int, [C.c_int, C.c_int]),
     "adaptq_kernel_launches": (C.c_ulonglong, []),
     "adaptq_last_attention_kernel": (C.c_char_p, []),

@@ -6,7 +6,8 @@ import shutil
 import subprocess
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(_HERE, "csrc", "adaptq_b200.cu")
+UNITS = [os.path.join(_HERE, "csrc", f) for f in ("adaptq_b200.cu", "paged.cu")]
+OBJ = os.path.join(_HERE, "obj")
 LIB = os.path.join(_HERE, "libadaptq_b200.so")
 # the same sources with -DADAPTQ_CHECKED: device-side index checks that record a status
 # instead of trapping, guard bytes behind every device buffer (see csrc/common.cuh)
@@ -34,20 +35,43 @@ def is_stale(lib: str = LIB) -> bool:
     return any(os.path.getmtime(s) > t for s in sources())
 
 
+def _object_is_stale(obj: str) -> bool:
+    """Older than anything of this repository that its translation unit includes (from the compiler's list)."""
+    dep = obj + ".d"
+    if not (os.path.exists(obj) and os.path.exists(dep)):
+        return True
+    with open(dep) as f:
+        names = f.read().replace("\\\n", " ").split(":", 1)[1].split()
+    root, t = os.path.dirname(_HERE) + os.sep, os.path.getmtime(obj)
+    mine = [n for n in map(os.path.abspath, names) if n.startswith(root)]
+    return any(not os.path.exists(n) or os.path.getmtime(n) > t for n in mine)
+
+
 def build_library(force: bool = False, verbose: bool = False, checked: bool = False) -> str:
     """nvcc -gencode arch=compute_100a,code=sm_100a ... -> libadaptq_b200.so
-    (checked=True: libadaptq_b200_checked.so, compiled with -DADAPTQ_CHECKED)"""
+    (checked=True: libadaptq_b200_checked.so, compiled with -DADAPTQ_CHECKED).  The translation
+    units are compiled side by side."""
     lib = LIB_CHECKED if checked else LIB
     if not force and not is_stale(lib):
         return lib
-    cmd = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "-Xcompiler", "-fPIC", "-shared", "-diag-suppress", "1886", "-o", lib, SRC]
+    os.makedirs(OBJ, exist_ok=True)
+    arch = ["-gencode", "arch=compute_100a,code=sm_100a"]
+    flags = [*arch, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-diag-suppress", "1886"]
     if checked:
-        cmd.insert(1, "-DADAPTQ_CHECKED=1")
+        flags.append("-DADAPTQ_CHECKED=1")
     if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    subprocess.check_call(cmd)
+        flags += ["-Xptxas", "-v"]
+    objects, running = [], []
+    for src in UNITS:
+        obj = os.path.join(OBJ, os.path.basename(src) + (".checked.o" if checked else ".o"))
+        objects.append(obj)
+        if force or _object_is_stale(obj):
+            cmd = [_nvcc(), *flags, "-MD", "-MF", obj + ".d", "-c", "-o", obj, src]
+            running.append((cmd, subprocess.Popen(cmd)))
+    failed = [(p.returncode, cmd) for cmd, p in running if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(*failed[0])
+    subprocess.check_call([_nvcc(), *arch, "-Xcompiler", "-fPIC", "-shared", "-o", lib, *objects])
     return lib
 
 

@@ -1844,5 +1844,17 @@ int adaptq_mha_compute_all_static(adaptq_mha_t h, const float *queries, int quer
 
 } // extern "C"
 
+#include "host_common.h"
+void aq_set_error(const char *fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(tl_error, sizeof(tl_error), fmt, ap);
+  va_end(ap);
+}
+void aq_clear_error() { clear_error(); }
+void aq_count_launch() { ++g_launches; }
+cudaError_t aq_launch_status() { return launch_status(); }
+void aq_sign_words(uint64_t seed, int padded, uint32_t *words, int n_words) { sign_words_for(seed, padded, words, n_words); }
+
 #include "runtime_v2_host.inc"
 #include "stack_host.inc"

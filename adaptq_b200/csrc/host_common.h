@@ -1,0 +1,13 @@
+// What the library's translation units share on the host side (defined in adaptq_b200.cu):
+// the calling thread's error string, the launch count, the failure seam and the sign generator.
+#pragma once
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#define AQ_HIDDEN __attribute__((visibility("hidden")))
+
+AQ_HIDDEN void aq_set_error(const char *fmt, ...);
+AQ_HIDDEN void aq_clear_error();
+AQ_HIDDEN void aq_count_launch();
+AQ_HIDDEN cudaError_t aq_launch_status(); // of the launch just made, or an injected failure
+AQ_HIDDEN void aq_sign_words(uint64_t seed, int padded, uint32_t *words, int n_words);

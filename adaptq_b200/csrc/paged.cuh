@@ -1,0 +1,118 @@
+// What the kernels of the paged cache share: the pool's geometry, 16- and 32-bit rows in and
+// out, rotary phases, and where a token lies.
+#pragma once
+#include "common.cuh"
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace aq {
+
+enum { TYPE_F32 = 0, TYPE_F16 = 1, TYPE_BF16 = 2 };
+enum { PAGED_BAD_PAGE = 1, PAGED_BAD_POSITION = 2, PAGED_GAVE_UP = 4 };
+
+struct PagedView {
+  uint8_t *k_pages, *v_pages;
+  float *k_scales, *v_scales;
+  const uint32_t *signs;
+  int *status;
+  long long n_pages;
+  int heads, page_size, page_shift, dim;
+};
+
+struct RotaryView { // dim == 0: no rotation
+  const unsigned long long *turns;
+  float factor;
+  int dim, interleaved;
+};
+
+struct TableView {
+  const int *entries;
+  long long stride;
+  int width;
+};
+
+// cos and sin of position * w, times the factor.  The frequency is a 64-bit binary fraction of
+// a turn, so the product modulo 2^64 is the phase modulo one turn, exact at every position;
+// only its last rounding, to 24 bits of half a turn, is left (1e-7 absolute in the angle).
+__device__ __forceinline__ float2 rotary_turn(const RotaryView &r, int pair, long long pos) {
+  const long long phase = (long long)((unsigned long long)pos * r.turns[pair]);
+  float s, c;
+  sincospif((float)phase * 0x1p-63f, &s, &c); // phase / 2^63 half turns, in [-1, 1)
+  return make_float2(c * r.factor, s * r.factor);
+}
+
+// One element of a rotated pair: mine * cos -+ other * sin (minus for the pair's first element).  One order of
+// rounding everywhere, so that a row does not depend on which kernel or layout rotates it.
+__device__ __forceinline__ float rotary_first(float mine, float other, float2 k) { return __fmaf_rn(mine, k.x, -__fmul_rn(other, k.y)); }
+__device__ __forceinline__ float rotary_second(float mine, float other, float2 k) { return __fmaf_rn(mine, k.x, __fmul_rn(other, k.y)); }
+
+__device__ __forceinline__ float load_one(const void *p, long long i, int type) {
+  if (type == TYPE_F32) return static_cast<const float *>(p)[i];
+  if (type == TYPE_F16) return __half2float(static_cast<const __half *>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+__device__ __forceinline__ void store_one(void *p, long long i, int type, float v) {
+  if (type == TYPE_F32) static_cast<float *>(p)[i] = v;
+  else if (type == TYPE_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ float2 unpack2(uint32_t w, int type) {
+  if (type == TYPE_F16) { __half2 h; memcpy(&h, &w, 4); return __half22float2(h); }
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, int type) {
+  uint32_t w;
+  if (type == TYPE_F16) { const __half2 h = __floats2half2_rn(a, b); memcpy(&w, &h, 4); }
+  else { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); memcpy(&w, &h, 4); }
+  return w;
+}
+
+// Eight consecutive elements; the address is 16-byte aligned.
+__device__ __forceinline__ void load_eight(const void *p, long long i, int type, float *v) {
+  if (type == TYPE_F32) {
+    const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+    const float4 b = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack2(u[j], type);
+      v[2 * j] = f.x; v[2 * j + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ void store_eight(void *p, long long i, int type, const float *v) {
+  if (type == TYPE_F32) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4 *>(static_cast<float *>(p) + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) =
+        make_uint4(pack2(v[0], v[1], type), pack2(v[2], v[3], type), pack2(v[4], v[5], type), pack2(v[6], v[7], type));
+  }
+}
+
+// Page and place of position `pos` of a sequence whose table row is `row`; false (and a bit
+// of the status) if the table or the pool has no such place.
+__device__ __forceinline__ bool find_slot(const PagedView &c, const int *row, int width, long long pos, int &page, int &off) {
+  if (pos < 0 || (pos >> c.page_shift) >= width) { atomicOr(c.status, PAGED_BAD_POSITION); return false; }
+  page = row[pos >> c.page_shift];
+  off = (int)(pos & (c.page_size - 1));
+  if (page < 0 || page >= c.n_pages) { atomicOr(c.status, PAGED_BAD_PAGE); return false; }
+  return true;
+}
+
+// The sequence of token t: the last b with cu[b] <= t, if t lies before cu[b+1].
+__device__ __forceinline__ int owner_of(const int *cu, int n_seqs, long long t) {
+  int lo = 0, hi = n_seqs; // cu[lo] <= t wanted, cu[hi] > t wanted
+  if (cu[0] > t || cu[n_seqs] <= t) return -1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+} // namespace aq

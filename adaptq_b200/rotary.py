@@ -1,0 +1,148 @@
+"""Rotary: rotary positions on CUDA tensors (include/adaptq_paged.h: adaptq_rotary_apply).
+
+The same object rotates the queries and keys that a caller handles itself, and goes along with
+PagedKVCache.append and .attend, which rotate on the way.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _inverse_frequencies(dim, base, scaling):
+    """([dim/2] angles per position in float64, factor of the rotated vector)."""
+    i = torch.arange(0, dim, 2, dtype=torch.float64) / dim
+    if scaling is None:
+        return base ** -i, 1.0
+    scaling = dict(scaling)
+    kind = scaling.pop("type", None)
+    known = {"linear": ("factor",), "ntk": ("factor",),
+             "yarn": ("factor", "original_max_position", "beta_fast", "beta_slow", "attention_factor"),
+             "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position")}
+    if kind not in known:
+        raise ValueError(f"scaling type must be one of {sorted(known)}, got {kind!r}")
+    extra = set(scaling) - set(known[kind])
+    if extra:
+        raise ValueError(f"unknown entries for {kind} scaling: {sorted(extra)}")
+    if not float(scaling.get("factor", 0.0)) > 0.0:
+        raise ValueError("scaling needs a positive factor")
+    factor = float(scaling["factor"])
+    if kind == "linear":
+        return base ** -i / factor, 1.0
+    if kind == "ntk":
+        if dim == 2:
+            raise ValueError("ntk scaling needs a rotary dimension above 2")
+        return (base * factor ** (dim / (dim - 2))) ** -i, 1.0
+    w = base ** -i
+    if not scaling.get("original_max_position", 0) > 0:
+        raise ValueError(f"{kind} scaling needs original_max_position")
+    old = float(scaling["original_max_position"])
+    if kind == "llama3":
+        low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+        if not high > low > 0.0:
+            raise ValueError("llama3 scaling needs high_freq_factor > low_freq_factor > 0")
+        wave = 2 * math.pi / w
+        smooth = (old / wave - low) / (high - low)
+        mid = (1 - smooth) * w / factor + smooth * w
+        return torch.where(wave > old / low, w / factor, torch.where(wave < old / high, w, mid)), 1.0
+    fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+    if not (fast > 0.0 and slow > 0.0 and base > 1.0):
+        raise ValueError("yarn scaling needs positive betas and a base above 1")
+    at = lambda turns: dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+    first, last = max(0, math.floor(at(fast))), min(dim - 1, math.ceil(at(slow)))
+    ramp = ((torch.arange(dim // 2, dtype=torch.float64) - first) / max(last - first, 0.001)).clamp(0, 1)
+    attention = scaling.get("attention_factor")
+    if attention is None:
+        attention = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    return w / factor * ramp + w * (1 - ramp), float(attention)
+
+
+class Rotary:
+    """Rotation of the first `dim` coordinates of a head by its position.
+
+    Pair i is (x[i], x[i + dim/2]), or (x[2i], x[2i+1]) if `interleaved`, and turns by
+    position * base^(-2i/dim).  `scaling` for contexts longer than a model was trained on:
+    None, or a dict with "type" and
+
+      linear   factor                       all angles divided by it
+      ntk      factor                       base * factor^(dim/(dim-2))
+      yarn     factor, original_max_position, [beta_fast 32, beta_slow 1, attention_factor]
+               slow pairs divided, fast ones kept, a ramp between; the vector is multiplied
+               by attention_factor (0.1 ln(factor) + 1)
+      llama3   factor, original_max_position, [low_freq_factor 1, high_freq_factor 4]
+
+    Angles are 64-bit fractions of a turn, so a position's phase is exact however far it is.
+    """
+
+    def __init__(self, dim: int, base: float = 10000.0, interleaved: bool = False, scaling=None, device=None):
+        if dim < 2 or dim % 2 or dim > 8192:
+            raise ValueError(f"the rotary dimension must be even, from 2 to 8192, got {dim}")
+        if not base > 0.0:
+            raise ValueError("base must be positive")
+        self.dim, self.base, self.interleaved = int(dim), float(base), bool(interleaved)
+        self.scaling = None if scaling is None else dict(scaling)
+        self.inv_freq, self.factor = _inverse_frequencies(self.dim, self.base, self.scaling)
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ValueError(f"Rotary needs a CUDA device, got {device}")
+        self._L = _lib.load()
+        turns = [int(w / (2 * math.pi) * 2.0 ** 64) % 2 ** 64 for w in self.inv_freq.tolist()]
+        self._turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
+        self.device = self._turns.device
+        self._desc = _lib.RotaryDesc(self._turns.data_ptr(), self.factor, self.dim, int(self.interleaved))
+        self._ref = C.addressof(self._desc)
+
+    def __call__(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor = None) -> torch.Tensor:
+        """x [tokens, heads, dim >= self.dim] (float32, float16 or bfloat16; any strides, the last one 1), positions
+        [tokens] (int32 or int64) -> the same shape and type.  `out` may be x (in place).  Differentiable in x (without
+        `out`)."""
+        if x.requires_grad and torch.is_grad_enabled():
+            if out is not None:
+                raise ValueError("out cannot be given for an x that requires a gradient")
+            return _Rotate.apply(x, positions, self)
+        return self._apply(x.detach(), positions, out, 0)
+
+    def _apply(self, x, positions, out, inverse):
+        if x.dim() != 3 or x.dtype not in TYPES or x.device != self.device:
+            raise ValueError(f"x must be (tokens, heads, dim) float32, float16 or bfloat16 on {self.device}, got {tuple(x.shape)} "
+                             f"{x.dtype} on {x.device}")
+        n, heads, dim = x.shape
+        if dim < self.dim:
+            raise ValueError(f"x has {dim} coordinates a head, the rotation {self.dim}")
+        if positions.shape != (n,) or positions.dtype not in (torch.int32, torch.int64) or positions.device != self.device:
+            raise ValueError(f"positions must be ({n},) int32 or int64 on {self.device}, got {tuple(positions.shape)} "
+                             f"{positions.dtype} on {positions.device}")
+        if dim > 1 and x.stride(2) != 1:
+            x = x.contiguous()
+        if out is None:
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (dim > 1 and out.stride(2) != 1):
+            raise ValueError("out must have the shape, type and device of x and contiguous rows")
+        positions = positions.contiguous()
+        xs, ys = x.stride(), out.stride()
+        if self._L.adaptq_rotary_apply(self._ref, x.data_ptr(), xs[0], xs[1], out.data_ptr(), ys[0], ys[1], TYPES[x.dtype],
+                                       positions.data_ptr(), positions.dtype == torch.int64, n, heads, dim, inverse,
+                                       self.device.index, torch.cuda.current_stream(self.device).cuda_stream):
+            raise RuntimeError(_lib.last_error())
+        return out
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, rotary):
+        ctx.rotary = rotary
+        ctx.save_for_backward(positions)
+        return rotary._apply(x, positions, None, 0)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        positions, = ctx.saved_tensors
+        return ctx.rotary._apply(grad, positions, None, 1), None, None
