@@ -4,9 +4,12 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-UNITS = [os.path.join(_HERE, "csrc", f) for f in ("adaptq_b200.cu", "paged.cu")]
+# translation units: source, name of the object, defines
+UNITS = [("adaptq_b200.cu", "adaptq_b200", []), ("paged.cu", "paged", [])] + \
+        [("paged_attend.cu", f"paged_attend_k{k}v{v}", [f"-DAQ_KB={k}", f"-DAQ_VB={v}"]) for k in (4, 3, 2) for v in (4, 3, 2)]
 OBJ = os.path.join(_HERE, "obj")
 LIB = os.path.join(_HERE, "libadaptq_b200.so")
 # the same sources with -DADAPTQ_CHECKED: device-side index checks that record a status
@@ -61,16 +64,15 @@ def build_library(force: bool = False, verbose: bool = False, checked: bool = Fa
         flags.append("-DADAPTQ_CHECKED=1")
     if verbose:
         flags += ["-Xptxas", "-v"]
-    objects, running = [], []
-    for src in UNITS:
-        obj = os.path.join(OBJ, os.path.basename(src) + (".checked.o" if checked else ".o"))
-        objects.append(obj)
+    def compile_unit(unit):
+        src, name, defines = unit
+        obj = os.path.join(OBJ, name + (".checked.o" if checked else ".o"))
         if force or _object_is_stale(obj):
-            cmd = [_nvcc(), *flags, "-MD", "-MF", obj + ".d", "-c", "-o", obj, src]
-            running.append((cmd, subprocess.Popen(cmd)))
-    failed = [(p.returncode, cmd) for cmd, p in running if p.wait() != 0]
-    if failed:
-        raise subprocess.CalledProcessError(*failed[0])
+            subprocess.check_call([_nvcc(), *flags, *defines, "-MD", "-MF", obj + ".d", "-c", "-o", obj, os.path.join(_HERE, "csrc", src)])
+        return obj
+
+    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        objects = list(pool.map(compile_unit, UNITS))
     subprocess.check_call([_nvcc(), *arch, "-Xcompiler", "-fPIC", "-shared", "-o", lib, *objects])
     return lib
 

@@ -11,3 +11,11 @@ AQ_HIDDEN void aq_clear_error();
 AQ_HIDDEN void aq_count_launch();
 AQ_HIDDEN cudaError_t aq_launch_status(); // of the launch just made, or an injected failure
 AQ_HIDDEN void aq_sign_words(uint64_t seed, int padded, uint32_t *words, int n_words);
+// Counts a launch just made and reports its failure, if any, as the error of `fn`.
+inline bool aq_launched(const char *fn) {
+  aq_count_launch();
+  const cudaError_t e = aq_launch_status();
+  if (e == cudaSuccess) return true;
+  aq_set_error("%s: CUDA error: %s", fn, cudaGetErrorString(e));
+  return false;
+}

@@ -2,7 +2,7 @@
 #include "../../include/adaptq_paged.h"
 #include "../../include/adaptq.h"
 #include "host_common.h"
-#include "paged_attend.cuh"
+#include "paged_attend_host.h"
 #include "paged_rows.cuh"
 #include "rotary.cuh"
 
@@ -67,13 +67,7 @@ bool check_rotary(const char *fn, const adaptq_rotary_t *r, int dim, RotaryView 
 
 bool check_type(const char *fn, int type) { return type >= 0 && type <= 2 ? true : fail(fn, "type must be 0 (float32), 1 (float16) or 2 (bfloat16)"); }
 
-bool launched(const char *fn) {
-  aq_count_launch();
-  const cudaError_t e = aq_launch_status();
-  if (e == cudaSuccess) return true;
-  aq_set_error("%s: CUDA error: %s", fn, cudaGetErrorString(e));
-  return false;
-}
+bool launched(const char *fn) { return aq_launched(fn); }
 
 template <int P, int KB, int VB> void launch_rows(const RowsLaunch &a, bool append, cudaStream_t s) {
   const long long rows = a.n_tokens * a.c.heads;
@@ -117,6 +111,17 @@ int rows_call(const char *fn, bool append, const adaptq_paged_t *cache, void *k,
   else launch_rows_k<256>(a, cache->k_bits, cache->v_bits, append, s);
   return launched(fn) ? 0 : -1;
 }
+
+// The kernels of one pair of bit widths are a translation unit of their own (paged_attend.cu).
+typedef bool (*attend_unit_t)(const AttendCall &);
+const attend_unit_t attend_units[3][3] = {{aq_attend_2_2, aq_attend_2_3, aq_attend_2_4},
+                                          {aq_attend_3_2, aq_attend_3_3, aq_attend_3_4},
+                                          {aq_attend_4_2, aq_attend_4_3, aq_attend_4_4}};
+
+// float32: two parts throughout.  float16: queries and weights in two parts, four queries a pass, so that what is lost
+// on the way stays below the output's own rounding (one part: 1.7 times the error of a 32-bit evaluation that is rounded
+// once).  bfloat16: one part, eight queries a pass; its output rounding is eight times coarser.
+int attend_mode(int type) { return type == TYPE_F32 ? ATTEND_EXACT : type == TYPE_F16 ? ATTEND_SPLIT : ATTEND_EIGHT; }
 
 } // namespace
 
@@ -178,8 +183,15 @@ int adaptq_paged_read(const adaptq_paged_t *cache, void *k_out, int64_t k_token_
 }
 
 size_t adaptq_paged_attend_workspace(const adaptq_paged_t *cache, int n_seqs, int n_q_heads, int type) {
-  (void)cache; (void)n_seqs; (void)n_q_heads; (void)type;
-  return 16;
+  if (!cache || n_seqs < 0 || cache->dim < 33 || cache->dim > 256 || cache->k_bits < 2 || cache->k_bits > 4 || cache->v_bits < 2 || cache->v_bits > 4 ||
+      cache->n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % cache->n_kv_heads)
+    return 0;
+  size_t bytes = 0;
+  AttendLaunch a{};
+  a.n_seqs = n_seqs; a.group = n_q_heads / cache->n_kv_heads; a.c.heads = cache->n_kv_heads;
+  attend_units[cache->k_bits - 2][cache->v_bits - 2]({"adaptq_paged_attend_workspace", &a, padded_of(cache->dim), attend_mode(type), cache->device,
+                                                      nullptr, nullptr, &bytes});
+  return bytes;
 }
 
 int adaptq_paged_attend(const adaptq_paged_t *cache, const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
@@ -195,19 +207,20 @@ int adaptq_paged_attend(const adaptq_paged_t *cache, const void *q, int64_t q_se
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(fn, "scale must be positive and finite"), -1;
   if (n_seqs == 0) return 0;
   if (!q || !out || !table || !lengths) return fail(fn, "null pointer"), -1;
-  if (!workspace || workspace_bytes < adaptq_paged_attend_workspace(cache, n_seqs, n_q_heads, type)) return fail(fn, "the workspace is too small"), -1;
+  if (n_q_heads / cache->n_kv_heads > 65536) return fail(fn, "at most 65536 queries per KV head are supported"), -1;
+  if ((long long)n_seqs * n_q_heads > 0x3fffffff) return fail(fn, "too many sequences for one call"), -1;
   a.table = TableView{table, table_stride, table_width};
   a.lengths = lengths; a.q = q; a.out = out; a.q_seq = q_seq_stride; a.q_head = q_head_stride;
   a.out_seq = out_seq_stride; a.out_head = out_head_stride;
-  a.n_seqs = n_seqs; a.q_heads = n_q_heads; a.group = n_q_heads / cache->n_kv_heads; a.type = type; a.scale = scale;
-  a.workspace = static_cast<float *>(workspace);
+  a.n_seqs = n_seqs; a.group = n_q_heads / cache->n_kv_heads; a.type = type; a.scale = scale;
   a.q_vec = vector_rows(q, q_seq_stride, q_head_stride, cache->dim, type);
   a.out_vec = vector_rows(out, out_seq_stride, out_head_stride, cache->dim, type);
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < adaptq_paged_attend_workspace(cache, n_seqs, n_q_heads, type))
+    return fail(fn, "the workspace is too small or not 16-byte aligned"), -1;
   DeviceScope dev(cache->device);
   if (!dev.ok) return fail(fn, "no usable CUDA device (this library has no CPU path)"), -1;
-  if ((long long)n_seqs * n_q_heads > 0x7fffffff) return fail(fn, "too many sequences for one call"), -1;
-  paged_attend_kernel<<<n_seqs * n_q_heads, ATTEND_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a, padded_of(cache->dim), cache->k_bits, cache->v_bits);
-  return launched(fn) ? 0 : -1;
+  const AttendCall call{fn, &a, padded_of(cache->dim), attend_mode(type), cache->device, workspace, static_cast<cudaStream_t>(stream), nullptr};
+  return attend_units[cache->k_bits - 2][cache->v_bits - 2](call) ? 0 : -1;
 }
 
 } // extern "C"
