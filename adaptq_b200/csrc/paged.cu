@@ -70,10 +70,20 @@ bool check_type(const char *fn, int type) { return type >= 0 && type <= 2 ? true
 bool launched(const char *fn) { return aq_launched(fn); }
 
 template <int P, int KB, int VB> void launch_rows(const RowsLaunch &a, bool append, cudaStream_t s) {
-  const long long rows = a.n_tokens * a.c.heads;
-  const dim3 grid((unsigned)((rows + rows_per_block<P> - 1) / rows_per_block<P>), 2);
-  if (append) paged_append_kernel<P, KB, VB><<<grid, ROWS_THREADS, 0, s>>>(a);
-  else paged_read_kernel<P, KB, VB><<<grid, ROWS_THREADS, 0, s>>>(a);
+  if (append) {
+    // the turns of a tile's tokens take 24 KB at most: smaller tiles where few heads share a token
+    const auto tokens = [&](int rows) { return std::min(rows, (rows + a.c.heads - 2) / a.c.heads + 1); };
+    RowsLaunch b = a;
+    for (b.tile_rows = rows_per_block<P>; tokens(b.tile_rows) * (a.r.dim / 2) * sizeof(float2) > 24576;) b.tile_rows /= 2;
+    const long long tiles = (a.n_tokens * a.c.heads + b.tile_rows - 1) / b.tile_rows;
+    // a block takes several tiles where there are many: its set-up is paid once
+    const unsigned blocks = (unsigned)std::min(tiles, std::max(1184ll, (tiles + 7) / 8));
+    paged_append_kernel<P, KB, VB><<<dim3(blocks, 2), ROWS_THREADS, (size_t)tokens(b.tile_rows) * (a.r.dim / 2) * sizeof(float2), s>>>(b);
+  } else {
+    const long long tiles = (a.n_tokens + 15) / 16;
+    const int shares = (a.c.heads + READ_WARPS - 1) / READ_WARPS;
+    paged_read_kernel<P, KB, VB><<<dim3((unsigned)tiles, 2, std::min(shares, 64)), READ_WARPS * 32, 0, s>>>(a);
+  }
 }
 template <int P, int KB> void launch_rows_v(const RowsLaunch &a, int vb, bool append, cudaStream_t s) {
   if (vb == 2) launch_rows<P, KB, 2>(a, append, s);

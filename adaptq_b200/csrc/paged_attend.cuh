@@ -85,11 +85,6 @@ __host__ __device__ constexpr float table_scale(int bits) { return bits == 2 ? 1
 
 enum { SEG_FROM_BEFORE = 1, SEG_ENDS = 2, SEG_OPEN = 4 }; // header flags: slot 0 in use, its item ends here, slot 1 in use
 
-__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -138,57 +133,10 @@ template <int WIDTH, int SHIFT> __device__ __forceinline__ uint32_t entry_addres
   else if constexpr (WIDTH == 6 && SHIFT == 7) return __dp4a(w, 0x80u << pos, base); // fields spread to bytes
   else return ((pos >= SHIFT ? w >> (pos - SHIFT) : w << (SHIFT - pos)) & (((1u << WIDTH) - 1) << SHIFT)) + base;
 }
-__device__ __forceinline__ uint32_t table_one(uint32_t at) {
-  uint32_t v;
-  asm("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
-  return v;
-}
 __device__ __forceinline__ uint2 table_two(uint32_t at) {
   uint2 v;
   asm("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
   return v;
-}
-
-// N packed bytes of a row -> words (bytes in memory order); the address is a multiple of the largest power of two in N.
-template <int N> __device__ __forceinline__ void load_packed(const uint8_t *p, uint32_t *w) {
-  if constexpr (N % 16 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 16; ++i) {
-      const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
-  } else if constexpr (N % 8 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 8; ++i) {
-      const uint2 v = reinterpret_cast<const uint2 *>(p)[i];
-      w[2 * i] = v.x; w[2 * i + 1] = v.y;
-    }
-  } else if constexpr (N % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-  } else if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      const uint32_t h = reinterpret_cast<const uint16_t *>(p)[i];
-      if (i & 1) w[i >> 1] |= h << 16; else w[i >> 1] = h;
-    }
-  } else {
-    w[0] = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[0] |= (uint32_t)p[i] << (8 * i);
-  }
-}
-// Four fields of six bits -> the lower six bits of four bytes.
-__device__ __forceinline__ uint32_t spread6(uint32_t v) {
-  v += (v & 0xfff000u) * 15u;      // each half of twelve bits in sixteen
-  return v + (v & 0x0fc00fc0u) * 3u; // each field in eight
-}
-// The g-th group of three bytes as a 24-bit number, first byte on top (3-bit rows).
-template <int WORDS> __device__ __forceinline__ uint32_t group24(const uint32_t (&w)[WORDS], int g) {
-  const int at = 3 * g, lo = at >> 2, o = at & 3;
-  const uint32_t next = lo + 1 < WORDS ? w[lo + 1 < WORDS ? lo + 1 : 0] : 0;
-  // bytes o, o+1, o+2 of (w[lo], next), reversed
-  return __byte_perm(w[lo], next, (o + 2) | ((o + 1) << 4) | (o << 8) | (o << 12)) & 0xffffffu;
 }
 
 // One query's sum of weighted values (coordinates lane*P/32 .. of the transformed domain) and of weights -> its output row.

@@ -1,8 +1,9 @@
 // Rows into the pages and out of them.
 //
-// One row of P coordinates is held by P/32 lanes, 32 consecutive coordinates each: five of the
-// log2 P butterfly stages stay inside a lane, the others are shuffles, and a lane's codes are a
-// whole number of words (4, 3 or 2).
+// Append: a row of P coordinates is held by P/32 lanes, 32 consecutive ones each, two in a
+// register pair (the float2 instructions round each half like the scalar ones): five of the
+// log2 P butterfly stages stay inside a lane, the others are shuffles, and a lane's codes are
+// a whole number of words.  Read-back: see paged_read_kernel.
 #pragma once
 #include "paged.cuh"
 
@@ -21,6 +22,7 @@ struct RowsLaunch {
   // the model's rows: keys and values (read by the append, written by the read-back)
   void *k, *v;
   long long k_token, k_head, v_token, v_head;
+  int tile_rows;          // rows of a tile of the append
   int type, k_vec, v_vec; // vec: rows 16-byte aligned, dim a multiple of 8
 };
 
@@ -40,68 +42,85 @@ template <int P> __device__ __forceinline__ void find_places(const RowsLaunch &a
   }
 }
 
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return __ffma2_rn(b, make_float2(-1.f, -1.f), a); }
+
 // Walsh-Hadamard butterflies over a row: 32 values a lane, P/32 lanes.
-template <int P> __device__ __forceinline__ void row_butterflies(float (&x)[32], int lane) {
+template <int P> __device__ __forceinline__ void row_butterflies(float2 (&x)[16], int lane) {
 #pragma unroll
-  for (int len = 1; len < 32; len <<= 1) {
+  for (int i = 0; i < 16; ++i) x[i] = make_float2(x[i].x + x[i].y, x[i].x - x[i].y);
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+  for (int len = 1; len < 16; len <<= 1) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
       if (!(i & len)) {
-        const float a = x[i], b = x[i + len];
-        x[i] = a + b;
-        x[i + len] = a - b;
+        const float2 a = x[i], b = x[i + len];
+        x[i] = add2(a, b);
+        x[i + len] = sub2(a, b);
       }
   }
 #pragma unroll
   for (int m = 1; m < P / 32; m <<= 1) {
-    const float sign = (lane & m) ? -1.f : 1.f;
+    const float s = (lane & m) ? -1.f : 1.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = fmaf(x[i], sign, __shfl_xor_sync(0xffffffffu, x[i], m));
+    for (int i = 0; i < 16; ++i) {
+      const float2 o = make_float2(__shfl_xor_sync(0xffffffffu, x[i].x, m), __shfl_xor_sync(0xffffffffu, x[i].y, m));
+      x[i] = __ffma2_rn(x[i], make_float2(s, s), o);
+    }
   }
 }
 
-__device__ __forceinline__ void flip_signs(float (&x)[32], uint32_t word) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(__float_as_uint(x[i]) ^ ((word << (31 - i)) & 0x80000000u));
+// Quantiser of 3 and 4 bits: the 128 buckets of a quarter from -16 on hold at most one threshold each, so a code is the
+// count of thresholds at or below the bucket's start and one comparison.  16 copies of the table, entry by entry, keep the
+// half-warps of a 64-bit read apart.  A coordinate is at most sqrt(P) = 16 in size.
+constexpr int BUCKETS = 128, BUCKET_COPIES = 16;
+template <int BITS> __device__ __forceinline__ void fill_buckets(uint2 *table, int tid) {
+  if (tid < BUCKETS) {
+    const float start = (tid - 64) * 0.25f;
+    float threshold = INFINITY;
+    uint32_t below = 0;
+    for (int i = (1 << BITS) - 2; i >= 0; --i) {
+      const float t = c_thr[BITS - 2][i];
+      if (t <= start) ++below;
+      else if (t < start + 0.25f) threshold = t;
+    }
+    for (int i = 0; i < BUCKET_COPIES; ++i) table[tid * BUCKET_COPIES + i] = make_uint2(__float_as_uint(threshold), below);
+  }
+}
+template <int P, int BITS> __device__ __forceinline__ uint32_t code_of(float u, const uint2 *table /* this lane's copy */) {
+  if constexpr (BITS == 2) return (uint32_t)quantize_value<2>(u);
+  else {
+    if constexpr (P == 256) u = fminf(fmaxf(u, -16.f), 15.75f);
+    const uint32_t bucket = __float_as_uint(__fmaf_rd(u, 4.f, 8388608.f + 64.f)) & (BUCKETS - 1); // floor(4 u) + 64; any of the table for NaN
+    const uint2 e = table[bucket * BUCKET_COPIES];
+    return e.y + (u >= __uint_as_float(e.x) ? 1u : 0u);
+  }
 }
 
-// 32 codes -> BITS words, most significant bits of each byte first.
-template <int BITS> __device__ __forceinline__ void pack_codes(const float (&u)[32], uint32_t (&w)[BITS]) {
+// 32 coordinates -> BITS words of codes, most significant bits of each byte first.
+template <int P, int BITS> __device__ __forceinline__ void pack_codes(const float2 (&u)[16], const uint2 *table, uint32_t (&w)[BITS]) {
+  auto code = [&](int i) { return code_of<P, BITS>((i & 1) ? u[i >> 1].y : u[i >> 1].x, table); };
   if constexpr (BITS == 3) {
     uint32_t r[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       uint32_t v = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v |= (uint32_t)quantize_value<3>(u[8 * g + i]) << (21 - 3 * i);
+      for (int i = 0; i < 8; ++i) v = v * 8 + code(8 * g + i);
       r[g] = __byte_perm(v, 0, 0x4012);
     }
     w[0] = r[0] | r[1] << 24;
     w[1] = r[1] >> 8 | r[2] << 16;
     w[2] = r[2] >> 16 | r[3] << 8;
   } else {
-    constexpr int PER = 32 / BITS, IN_BYTE = 8 / BITS;
+    constexpr int PER = 32 / BITS;
 #pragma unroll
     for (int g = 0; g < BITS; ++g) {
       uint32_t v = 0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        v |= (uint32_t)quantize_value<BITS>(u[PER * g + i]) << (8 * (i / IN_BYTE) + 8 - BITS * (1 + i % IN_BYTE));
-      w[g] = v;
+      for (int i = 0; i < PER; ++i) v = v * (1u << BITS) + code(PER * g + i); // first code on top
+      w[g] = __byte_perm(v, 0, 0x0123);
     }
-  }
-}
-
-template <int BITS> __device__ __forceinline__ int code_at(const uint32_t (&w)[BITS], int i) {
-  if constexpr (BITS == 3) { // bits 3i, 3i+1, 3i+2 of the row, bytes in memory order
-    const int g = i >> 3, at = 24 * g; // group of three bytes
-    const uint32_t lo = w[at >> 5] >> (at & 31), hi = (at & 31) ? w[min(2, (at >> 5) + 1)] << (32 - (at & 31)) : 0;
-    const uint32_t v = __byte_perm((at & 31) ? lo | hi : lo, 0, 0x4012);
-    return (v >> (21 - 3 * (i & 7))) & 7;
-  } else {
-    constexpr int PER = 32 / BITS, IN_BYTE = 8 / BITS;
-    const int j = i % PER;
-    return (w[i / PER] >> (8 * (j / IN_BYTE) + 8 - BITS * (1 + j % IN_BYTE))) & ((1 << BITS) - 1);
   }
 }
 
@@ -113,169 +132,236 @@ template <int BITS> __device__ __forceinline__ void store_words(uint8_t *p, cons
     for (int i = 0; i < 3; ++i) reinterpret_cast<uint32_t *>(p)[i] = w[i];
   }
 }
-template <int BITS> __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[BITS]) {
-  if constexpr (BITS == 4) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (BITS == 2) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    w[0] = v.x; w[1] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-  }
-}
-
+// One side of the append: tiles of up to rows_per_block rows, token by token.
 template <int P, int BITS>
 __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src, long long src_token, long long src_head,
                                             bool vec, uint8_t *pages, float *scales, bool rotate, float2 *turns,
-                                            TokenPlace *place) {
-  constexpr int LANES = P / 32, ROWS = rows_per_block<P>;
-  const int heads = a.c.heads, dim = a.c.dim, half = a.r.dim >> 1;
-  const long long n_rows = a.n_tokens * heads, r0 = (long long)blockIdx.x * ROWS;
-  const long long t0 = r0 / heads;
-  const int nt = (int)(min(n_rows - 1, r0 + ROWS - 1) / heads - t0) + 1;
+                                            TokenPlace *place, uint2 *table) {
+  constexpr int LANES = P / 32;
+  const int heads = a.c.heads, dim = a.c.dim, half = a.r.dim >> 1, ROWS = a.tile_rows;
+  const long long n_rows = a.n_tokens * heads;
   const int lane = threadIdx.x & 31, part = lane % LANES, d0 = part * 32;
-  long long row = r0 + threadIdx.x / LANES;
-  const bool live = row < n_rows;
-  if (!live) row = n_rows - 1;
-  const long long t = row / heads;
-  const int h = (int)(row - t * heads);
-  const long long at = t * src_token + h * src_head;
+  if constexpr (BITS != 2) fill_buckets<BITS>(table, threadIdx.x);
+  for (long long r0 = (long long)blockIdx.x * ROWS; r0 < n_rows; r0 += (long long)gridDim.x * ROWS) {
+    const long long t0 = r0 / heads;
+    const int in_first = (int)(r0 - t0 * heads); // rows of token t0 before this tile
+    const int live_rows = (int)min((long long)ROWS, n_rows - r0);
+    const int nt = (in_first + live_rows - 1) / heads + 1;
+    const int local = min((int)threadIdx.x / LANES, live_rows - 1);
+    const int dt = (in_first + local) / heads, h = in_first + local - dt * heads;
+    const bool live = threadIdx.x / LANES < live_rows;
+    const long long at = (t0 + dt) * src_token + h * src_head;
 
-  float x[32];
+    float2 x[16];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) x[i] = 0.f;
-  if (vec) {
+    for (int i = 0; i < 16; ++i) x[i] = make_float2(0.f, 0.f);
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      if (d0 + i < dim) load_eight(src, at + d0 + i, a.type, x + i);
-  } else {
+      for (int i = 0; i < 32; i += 8)
+        if (d0 + i < dim) {
+          float v[8];
+          load_eight(src, at + d0 + i, a.type, v);
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (d0 + i < dim) x[i] = load_one(src, at + d0 + i, a.type);
-  }
-  const uint32_t signs = a.c.signs[h * LANES + part];
-
-  find_places<P>(a, t0, nt, place);
-  __syncthreads();
-  if (rotate) {
-    for (int i = threadIdx.x; i < nt * half; i += ROWS_THREADS) turns[i] = rotary_turn(a.r, i % half, place[i / half].pos);
-    __syncthreads();
-    const float2 *cs = turns + (int)(t - t0) * half;
-    if (a.r.interleaved) {
-#pragma unroll
-      for (int i = 0; i < 32; i += 2)
-        if (d0 + i < a.r.dim) {
-          const float2 k = cs[(d0 + i) >> 1];
-          const float u = x[i], v = x[i + 1];
-          x[i] = rotary_first(u, v, k);
-          x[i + 1] = rotary_second(v, u, k);
+          for (int j = 0; j < 4; ++j) x[i / 2 + j] = make_float2(v[2 * j], v[2 * j + 1]);
         }
     } else {
-      // the partner of coordinate i is i +- half: in another lane's same place where half is a
-      // multiple of 32, else fetched again (from L1)
-      const bool shuffle = (half & 31) == 0;
-      const int m = half >> 5, from = part < m ? part + m : part < 2 * m ? part - m : part;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int d = d0 + i;
-        const bool first = d < half, in = d < a.r.dim;
-        float other = 0.f;
-        if (shuffle) other = __shfl_sync(0xffffffffu, x[i], (lane & ~(LANES - 1)) + from);
-        else if (in) other = load_one(src, at + (first ? d + half : d - half), a.type);
-        if (in) {
-          const float2 k = cs[first ? d : d - half];
-          x[i] = first ? rotary_first(x[i], other, k) : rotary_second(x[i], other, k);
+      for (int i = 0; i < 16; ++i) {
+        if (d0 + 2 * i < dim) x[i].x = load_one(src, at + d0 + 2 * i, a.type);
+        if (d0 + 2 * i + 1 < dim) x[i].y = load_one(src, at + d0 + 2 * i + 1, a.type);
+      }
+    }
+    const uint32_t signs = a.c.signs[h * LANES + part];
+
+    __syncthreads(); // the previous tile's places and turns have been used
+    find_places<P>(a, t0, nt, place);
+    __syncthreads();
+    if (rotate) {
+      for (int i = threadIdx.x; i < nt * half; i += ROWS_THREADS) turns[i] = rotary_turn(a.r, i % half, place[i / half].pos);
+      __syncthreads();
+      const float2 *cs = turns + dt * half;
+      if (a.r.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (d0 + 2 * i < a.r.dim) {
+            const float2 k = cs[(d0 >> 1) + i];
+            x[i] = make_float2(rotary_first(x[i].x, x[i].y, k), rotary_second(x[i].y, x[i].x, k));
+          }
+      } else {
+        // the partner of coordinate i is i +- half: in another lane's same place where half is a
+        // multiple of 32, else fetched again (from L1)
+        const bool shuffle = (half & 31) == 0;
+        const int m = half >> 5, from = (lane & ~(LANES - 1)) + (part < m ? part + m : part < 2 * m ? part - m : part);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int d = d0 + i;
+          const bool first = d < half, in = d < a.r.dim;
+          float &v = (i & 1) ? x[i >> 1].y : x[i >> 1].x;
+          float other = 0.f;
+          if (shuffle) other = __shfl_sync(0xffffffffu, v, from);
+          else if (in) other = load_one(src, at + (first ? d + half : d - half), a.type);
+          if (in) {
+            const float2 k = cs[first ? d : d - half];
+            v = first ? rotary_first(v, other, k) : rotary_second(v, other, k);
+          }
         }
       }
     }
-  }
 
-  float sum = 0.f;
+    float2 sum2 = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) sum = fmaf(x[i], x[i], sum);
+    for (int i = 0; i < 16; ++i) sum2 = __ffma2_rn(x[i], x[i], sum2);
+    float sum = sum2.x + sum2.y;
 #pragma unroll
-  for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-  const float norm = sqrtf(sum + 1e-12f), inv = 1.f / norm;
-  // the transform first, the norm after it: sums of 16-bit values that are zero (a threshold) stay zero
-  flip_signs(x, signs);
-  row_butterflies<P>(x, lane);
+    for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    const float norm = sqrtf(sum + 1e-12f), inv = 1.f / norm;
+    // the transform first, the norm after it: sums of 16-bit values that are zero (a threshold) stay zero
 #pragma unroll
-  for (int i = 0; i < 32; ++i) x[i] *= inv;
-  uint32_t w[BITS];
-  pack_codes<BITS>(x, w);
+    for (int i = 0; i < 16; ++i) {
+      x[i].x = __uint_as_float(__float_as_uint(x[i].x) ^ ((signs << (31 - 2 * i)) & 0x80000000u));
+      x[i].y = __uint_as_float(__float_as_uint(x[i].y) ^ ((signs << (30 - 2 * i)) & 0x80000000u));
+    }
+    row_butterflies<P>(x, lane);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = __fmul2_rn(x[i], make_float2(inv, inv));
+    uint32_t w[BITS];
+    pack_codes<P, BITS>(x, table + (lane & (BUCKET_COPIES - 1)), w);
 
-  const TokenPlace p = place[(int)(t - t0)];
-  if (live && p.page >= 0) {
-    const long long slot = (((long long)p.page * heads + h) << a.c.page_shift) + p.off;
-    store_words<BITS>(pages + slot * (P * BITS / 8) + part * (4 * BITS), w);
-    if (part == 0) scales[slot] = norm;
+    const TokenPlace p = place[dt];
+    if (live && p.page >= 0) {
+      const long long slot = (((long long)p.page * heads + h) << a.c.page_shift) + p.off;
+      store_words<BITS>(pages + slot * (P * BITS / 8) + part * (4 * BITS), w);
+      if (part == 0) scales[slot] = norm;
+    }
   }
 }
 
-// blockIdx.y: 0 = keys, 1 = values
+// blockIdx.y: 0 = keys, 1 = values.  Dynamic shared memory: the turns of a tile's tokens.
 template <int P, int KB, int VB> __global__ void __launch_bounds__(ROWS_THREADS) paged_append_kernel(const RowsLaunch a) {
-  __shared__ float2 turns[rows_per_block<P> * P / 2];
+  extern __shared__ float2 turns[];
+  __shared__ uint2 table[BUCKETS * BUCKET_COPIES];
   __shared__ TokenPlace place[rows_per_block<P>];
   if (blockIdx.y == 0)
-    append_rows<P, KB>(a, a.k, a.k_token, a.k_head, a.k_vec, a.c.k_pages, a.c.k_scales, a.r.dim > 0, turns, place);
+    append_rows<P, KB>(a, a.k, a.k_token, a.k_head, a.k_vec, a.c.k_pages, a.c.k_scales, a.r.dim > 0, turns, place, table);
   else
-    append_rows<P, VB>(a, a.v, a.v_token, a.v_head, a.v_vec, a.c.v_pages, a.c.v_scales, false, turns, place);
+    append_rows<P, VB>(a, a.v, a.v_token, a.v_head, a.v_vec, a.c.v_pages, a.c.v_scales, false, turns, place, table);
 }
+
+// Read-back.  A warp takes 16 tokens of one head.  A code becomes the pair {upper, lower} of float16 parts of its
+// codebook value, which is one register of the first operand of mma.sync m16n8k16: the contracted dimension holds both parts
+// of eight codes, the second operand the signs of a Walsh-Hadamard transform of eight (twice, once for each part).  Lane
+// (g, t) holds the coordinates t*P/4 .. of the rows g and g+8; the eight of a step are {t*P/4 + 2s + i}, i < 2, so
+// the product transforms along t and i, and log2(P/8) stages of butterflies along s remain inside the lane.  22 bits
+// of the codebook and float32 sums: as exact as the butterflies alone, which cost three times the instructions.
+template <int BITS> __device__ __forceinline__ uint32_t code_bytes(const uint32_t *w, int i, const uint32_t *g24) {
+  // a word that holds code i in its byte (see code_byte)
+  if constexpr (BITS == 4) return (i & 1) ? w[i >> 3] & 0x0f0f0f0fu : (w[i >> 3] >> 4) & 0x0f0f0f0fu;
+  else if constexpr (BITS == 2) return (w[i >> 4] >> (6 - 2 * (i & 3))) & 0x03030303u;
+  else return (i & 1) ? g24[i >> 3] & 0x07070707u : (g24[i >> 3] >> 3) & 0x07070707u;
+}
+template <int BITS> __device__ __forceinline__ constexpr int code_byte(int i) { return BITS == 4 ? (i >> 1) & 3 : BITS == 2 ? (i >> 2) & 3 : 3 - ((i >> 1) & 3); }
+
+constexpr int READ_WARPS = 8;
 
 template <int P, int BITS>
 __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long long dst_token, long long dst_head, bool vec,
-                                          const uint8_t *pages, const float *scales, float (*level)[32], TokenPlace *place) {
-  constexpr int LANES = P / 32, ROWS = rows_per_block<P>;
-  const int heads = a.c.heads, dim = a.c.dim;
-  const long long n_rows = a.n_tokens * heads, r0 = (long long)blockIdx.x * ROWS;
-  const long long t0 = r0 / heads;
-  const int nt = (int)(min(n_rows - 1, r0 + ROWS - 1) / heads - t0) + 1;
-  const int lane = threadIdx.x & 31, part = lane % LANES, d0 = part * 32;
-  long long row = r0 + threadIdx.x / LANES;
-  const bool live = row < n_rows;
-  if (!live) row = n_rows - 1;
-  const long long t = row / heads;
-  const int h = (int)(row - t * heads);
+                                          const uint8_t *pages, const float *scales, uint32_t (*level)[32], TokenPlace *place) {
+  constexpr int N = P / 4, S = N / 2, WORDS = (N * BITS / 8 + 3) / 4;
+  const int heads = a.c.heads, dim = a.c.dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long t0 = (long long)blockIdx.x * 16;
+  const int nt = (int)min(16ll, a.n_tokens - t0);
   // a copy of the codebook for every lane: 32 reads of any codes hit 32 banks
-  for (int i = threadIdx.x; i < (32 << BITS); i += ROWS_THREADS) level[i >> 5][i & 31] = c_cb[BITS - 2][i >> 5];
+  for (int i = threadIdx.x; i < (32 << BITS); i += READ_WARPS * 32) {
+    const float c = c_cb[BITS - 2][i >> 5], upper = __half2float(__float2half_rn(c));
+    level[i >> 5][i & 31] = pack2(upper, c - upper, TYPE_F16);
+  }
   find_places<P>(a, t0, nt, place);
   __syncthreads();
-  const TokenPlace p = place[(int)(t - t0)];
-  const bool found = p.page >= 0;
-  uint32_t w[BITS] = {};
-  float norm = 0.f;
-  if (found) {
-    const long long slot = (((long long)p.page * heads + h) << a.c.page_shift) + p.off;
-    load_words<BITS>(pages + slot * (P * BITS / 8) + part * (4 * BITS), w);
-    norm = scales[slot];
-  }
-  const uint32_t signs = a.c.signs[h * LANES + part];
-  float x[32];
+  const uint32_t mine = smem_u32(&level[0][lane]);
+  const int odd = __popc(t & (g >> 1)) & 1;
+  const uint32_t b0 = odd ? 0xbc00bc00u : 0x3c003c00u, b1 = odd ^ (g & 1) ? 0xbc00bc00u : 0x3c003c00u; // {1, 1} or {-1, -1}
+  TokenPlace p[2];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) x[i] = level[code_at<BITS>(w, i)][lane];
-  row_butterflies<P>(x, lane);
-  flip_signs(x, signs);
-  const float scale = norm * (1.f / P);
+  for (int r = 0; r < 2; ++r) p[r] = g + 8 * r < nt ? place[g + 8 * r] : TokenPlace{-1, 0, 0};
+  for (int h = blockIdx.z * READ_WARPS + warp; h < heads; h += gridDim.z * READ_WARPS) {
+    uint32_t w[2][WORDS], g24[2][BITS == 3 ? N / 8 : 1];
+    float scale[2];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) x[i] *= scale;
-  if (!live || !found) return;
-  const long long at = t * dst_token + h * dst_head;
-  if (vec) {
+    for (int r = 0; r < 2; ++r) {
+      scale[r] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      if (d0 + i < dim) store_eight(dst, at + d0 + i, a.type, x + i);
-  } else {
+      for (int i = 0; i < WORDS; ++i) w[r][i] = 0;
+      if (p[r].page >= 0) {
+        const long long slot = (((long long)p[r].page * heads + h) << a.c.page_shift) + p[r].off;
+        load_packed<N * BITS / 8>(pages + slot * (P * BITS / 8) + t * (N * BITS / 8), w[r]);
+        scale[r] = scales[slot] * (1.f / P);
+      }
+      if constexpr (BITS == 3) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (d0 + i < dim) store_one(dst, at + d0 + i, a.type, x[i]);
+        for (int i = 0; i < N / 8; ++i) g24[r][i] = spread6(group24<WORDS>(w[r], i));
+      }
+    }
+    float2 x[2][S]; // coordinates 2s, 2s+1 of this lane's part
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      uint32_t e[2][2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          e[r][i] = table_one(__dp4a(code_bytes<BITS>(w[r], 2 * s + i, g24[r]), 0x80u << (8 * code_byte<BITS>(2 * s + i)), mine));
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_16816(d, e[0][0], e[1][0], e[0][1], e[1][1], b0, b1);
+      x[0][s] = make_float2(d[0], d[1]);
+      x[1][s] = make_float2(d[2], d[3]);
+    }
+#pragma unroll
+    for (int len = 1; len < S; len <<= 1)
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (!(s & len)) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float2 u = x[r][s], v = x[r][s + len];
+            x[r][s] = add2(u, v);
+            x[r][s + len] = sub2(u, v);
+          }
+        }
+    const uint32_t *signs = a.c.signs + h * (P / 32) + ((t * N) >> 5);
+    const uint32_t word[2] = {signs[0] >> ((t * N) & 31), N > 32 ? signs[1] : 0u};
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const uint32_t bits = word[s >> 4], f0 = (bits << (31 - 2 * (s & 15))) & 0x80000000u, f1 = (bits << (30 - 2 * (s & 15))) & 0x80000000u;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t f = __float_as_uint(scale[r]);
+        x[r][s] = __fmul2_rn(x[r][s], make_float2(__uint_as_float(f ^ f0), __uint_as_float(f ^ f1)));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      if (p[r].page < 0) continue;
+      const long long at = (t0 + g + 8 * r) * dst_token + h * dst_head + t * N;
+      if (vec) {
+#pragma unroll
+        for (int i = 0; i < N; i += 8)
+          if (t * N + i < dim) {
+            const float v[8] = {x[r][i / 2].x, x[r][i / 2].y, x[r][i / 2 + 1].x, x[r][i / 2 + 1].y, x[r][i / 2 + 2].x, x[r][i / 2 + 2].y, x[r][i / 2 + 3].x, x[r][i / 2 + 3].y};
+            store_eight(dst, at + i, a.type, v);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (t * N + i < dim) store_one(dst, at + i, a.type, (i & 1) ? x[r][i >> 1].y : x[r][i >> 1].x);
+      }
+    }
   }
 }
 
-template <int P, int KB, int VB> __global__ void __launch_bounds__(ROWS_THREADS) paged_read_kernel(const RowsLaunch a) {
-  __shared__ float level[16][32];
-  __shared__ TokenPlace place[rows_per_block<P>];
+// Grid: 16 tokens, side (keys, values), share of the heads.
+template <int P, int KB, int VB> __global__ void __launch_bounds__(READ_WARPS * 32) paged_read_kernel(const RowsLaunch a) {
+  __shared__ uint32_t level[16][32];
+  __shared__ TokenPlace place[16];
   if (blockIdx.y == 0)
     read_rows<P, KB>(a, a.k, a.k_token, a.k_head, a.k_vec, a.c.k_pages, a.c.k_scales, level, place);
   else
