@@ -71,18 +71,21 @@ bool launched(const char *fn) { return aq_launched(fn); }
 
 template <int P, int KB, int VB> void launch_rows(const RowsLaunch &a, bool append, cudaStream_t s) {
   if (append) {
-    // the turns of a tile's tokens take 24 KB at most: smaller tiles where few heads share a token
-    const auto tokens = [&](int rows) { return std::min(rows, (rows + a.c.heads - 2) / a.c.heads + 1); };
+    constexpr int ROWS = rows_per_warp<P>, WARPS = ROWS_THREADS / 32;
     RowsLaunch b = a;
-    for (b.tile_rows = rows_per_block<P>; tokens(b.tile_rows) * (a.r.dim / 2) * sizeof(float2) > 24576;) b.tile_rows /= 2;
-    const long long tiles = (a.n_tokens * a.c.heads + b.tile_rows - 1) / b.tile_rows;
-    // a block takes several tiles where there are many: its set-up is paid once
-    const unsigned blocks = (unsigned)std::min(tiles, std::max(1184ll, (tiles + 7) / 8));
-    paged_append_kernel<P, KB, VB><<<dim3(blocks, 2), ROWS_THREADS, (size_t)tokens(b.tile_rows) * (a.r.dim / 2) * sizeof(float2), s>>>(b);
+    b.turn_tokens = std::min(ROWS, (ROWS + a.c.heads - 2) / a.c.heads + 1);
+    const long long passes = (a.n_tokens * a.c.heads + ROWS * WARPS - 1) / (ROWS * WARPS);
+    // a block takes several passes where there are many: its table is filled once
+    const unsigned blocks = (unsigned)std::min(passes, std::max(592ll, (passes + 15) / 16));
+    paged_append_kernel<P, KB, VB><<<dim3(blocks, 2), ROWS_THREADS, (size_t)WARPS * b.turn_tokens * a.r.dim * sizeof(float), s>>>(b);
   } else {
-    const long long tiles = (a.n_tokens + 15) / 16;
-    const int shares = (a.c.heads + READ_WARPS - 1) / READ_WARPS;
-    paged_read_kernel<P, KB, VB><<<dim3((unsigned)tiles, 2, std::min(shares, 64)), READ_WARPS * 32, 0, s>>>(a);
+    RowsLaunch b = a;
+    // blocks of 64 tokens, smaller ones where those would leave SMs without work
+    for (b.block_tokens = READ_TOKENS; b.block_tokens > 16 && 2 * ((a.n_tokens + b.block_tokens - 1) / b.block_tokens) < 592;) b.block_tokens /= 2;
+    const unsigned tiles = (unsigned)((a.n_tokens + b.block_tokens - 1) / b.block_tokens);
+    const long long items = (long long)(b.block_tokens / 16) * a.c.heads;
+    const unsigned shares = (unsigned)std::max(1ll, std::min((items + READ_WARPS - 1) / READ_WARPS, 592ll / (2 * tiles)));
+    paged_read_kernel<P, KB, VB><<<dim3(tiles, 2, shares), READ_WARPS * 32, 0, s>>>(b);
   }
 }
 template <int P, int KB> void launch_rows_v(const RowsLaunch &a, int vb, bool append, cudaStream_t s) {
@@ -107,12 +110,16 @@ int rows_call(const char *fn, bool append, const adaptq_paged_t *cache, void *k,
   if (n_seqs == 0 || n_tokens == 0) return 0;
   if (!k || !v || !table || !starts) return fail(fn, "null pointer"), -1;
   const int P = padded_of(cache->dim);
-  if (n_tokens > (1ll << 31) / cache->n_kv_heads * (ROWS_THREADS * 32 / P)) return fail(fn, "too many tokens for one call"), -1;
+  if (n_tokens > (1ll << 31) / cache->n_kv_heads) return fail(fn, "too many tokens for one call"), -1;
   a.table = TableView{table, table_stride, table_width};
   a.starts = starts; a.start_bias = start_bias; a.cu = cu_tokens; a.n_seqs = n_seqs; a.n_tokens = n_tokens;
   a.k = k; a.k_token = k_token; a.k_head = k_head; a.v = v; a.v_token = v_token; a.v_head = v_head; a.type = type;
   a.k_vec = vector_rows(k, k_token, k_head, cache->dim, type);
   a.v_vec = vector_rows(v, v_token, v_head, cache->dim, type);
+  const int per = 32 / size_of(type); // elements of a 32-byte store
+  const auto wide = [&](const void *p, int64_t s0, int64_t s1) { return aligned(p, 32) && s0 % per == 0 && s1 % per == 0 && cache->dim % 16 == 0; };
+  if (!append && a.k_vec && wide(k, k_token, k_head)) a.k_vec = 2;
+  if (!append && a.v_vec && wide(v, v_token, v_head)) a.v_vec = 2;
   DeviceScope dev(cache->device);
   if (!dev.ok) return fail(fn, "no usable CUDA device (this library has no CPU path)"), -1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

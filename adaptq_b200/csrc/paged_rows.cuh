@@ -10,7 +10,7 @@
 namespace aq {
 
 constexpr int ROWS_THREADS = 256;
-template <int P> constexpr int rows_per_block = ROWS_THREADS / (P / 32);
+template <int P> constexpr int rows_per_warp = 32 / (P / 32);
 
 struct RowsLaunch {
   PagedView c;
@@ -22,24 +22,22 @@ struct RowsLaunch {
   // the model's rows: keys and values (read by the append, written by the read-back)
   void *k, *v;
   long long k_token, k_head, v_token, v_head;
-  int tile_rows;          // rows of a tile of the append
-  int type, k_vec, v_vec; // vec: rows 16-byte aligned, dim a multiple of 8
+  int turn_tokens;        // append: tokens of a warp's rows at most
+  int block_tokens;       // read-back: tokens of a block
+  int type, k_vec, v_vec; // 0; 1: rows 16-byte aligned, dim a multiple of 8; 2: 32-byte aligned, a multiple of 16 as well
 };
 
 struct TokenPlace { int page, off; long long pos; }; // page < 0: nowhere
 
-// Places of the tokens that this block's rows belong to.
-template <int P> __device__ __forceinline__ void find_places(const RowsLaunch &a, long long t0, int nt, TokenPlace *place) {
-  for (int i = threadIdx.x; i < nt; i += ROWS_THREADS) {
-    const long long t = t0 + i;
-    const int b = a.cu ? owner_of(a.cu, a.n_seqs, t) : (t < a.n_seqs ? (int)t : -1);
-    TokenPlace p{-1, 0, 0};
-    if (b >= 0 && !(a.start_bias < 0 && a.starts[b] == 0)) { // a decode step leaves empty sequences out
-      p.pos = (long long)a.starts[b] + a.start_bias + (a.cu ? t - a.cu[b] : 0);
-      if (!find_slot(a.c, a.table.entries + b * a.table.stride, a.table.width, p.pos, p.page, p.off)) p.page = -1;
-    }
-    place[i] = p;
+// Where token t goes to, or is read from.
+__device__ __forceinline__ TokenPlace find_place(const RowsLaunch &a, long long t) {
+  const int b = a.cu ? owner_of(a.cu, a.n_seqs, t) : (t < a.n_seqs ? (int)t : -1);
+  TokenPlace p{-1, 0, 0};
+  if (b >= 0 && !(a.start_bias < 0 && a.starts[b] == 0)) { // a decode step leaves empty sequences out
+    p.pos = (long long)a.starts[b] + a.start_bias + (a.cu ? t - a.cu[b] : 0);
+    if (!find_slot(a.c, a.table.entries + b * a.table.stride, a.table.width, p.pos, p.page, p.off)) p.page = -1;
   }
+  return p;
 }
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
@@ -87,39 +85,47 @@ template <int BITS> __device__ __forceinline__ void fill_buckets(uint2 *table, i
     for (int i = 0; i < BUCKET_COPIES; ++i) table[tid * BUCKET_COPIES + i] = make_uint2(__float_as_uint(threshold), below);
   }
 }
-template <int P, int BITS> __device__ __forceinline__ uint32_t code_of(float u, const uint2 *table /* this lane's copy */) {
-  if constexpr (BITS == 2) return (uint32_t)quantize_value<2>(u);
+// word = word << BITS | code of u
+template <int P, int BITS> __device__ __forceinline__ void push_code(uint32_t &word, float u, const uint2 *table, uint32_t copy /* 8 * lane's copy */) {
+  if constexpr (BITS == 2) word = word * 4 + (uint32_t)quantize_value<2>(u);
   else {
     if constexpr (P == 256) u = fminf(fmaxf(u, -16.f), 15.75f);
-    const uint32_t bucket = __float_as_uint(__fmaf_rd(u, 4.f, 8388608.f + 64.f)) & (BUCKETS - 1); // floor(4 u) + 64; any of the table for NaN
-    const uint2 e = table[bucket * BUCKET_COPIES];
-    return e.y + (u >= __uint_as_float(e.x) ? 1u : 0u);
+    // 4 u + 64 in units of 2^-7, rounded down: the bucket lies where a byte offset into the table wants it (any for NaN)
+    const uint32_t at = (__float_as_uint(__fmaf_rd(u, 4.f, 65536.f + 64.f)) & ((BUCKETS - 1) << 7)) | copy;
+    const uint2 e = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint8_t *>(table) + at);
+    word = word * (1u << BITS) + e.y;
+    if (u >= __uint_as_float(e.x)) ++word;
   }
 }
 
 // 32 coordinates -> BITS words of codes, most significant bits of each byte first.
-template <int P, int BITS> __device__ __forceinline__ void pack_codes(const float2 (&u)[16], const uint2 *table, uint32_t (&w)[BITS]) {
-  auto code = [&](int i) { return code_of<P, BITS>((i & 1) ? u[i >> 1].y : u[i >> 1].x, table); };
+template <int P, int BITS> __device__ __forceinline__ void pack_codes(const float2 (&u)[16], const uint2 *table, uint32_t copy, uint32_t (&w)[BITS]) {
   if constexpr (BITS == 3) {
     uint32_t r[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       uint32_t v = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v = v * 8 + code(8 * g + i);
+      for (int i = 0; i < 4; ++i) {
+        push_code<P, BITS>(v, u[4 * g + i].x, table, copy);
+        push_code<P, BITS>(v, u[4 * g + i].y, table, copy);
+      }
       r[g] = __byte_perm(v, 0, 0x4012);
     }
     w[0] = r[0] | r[1] << 24;
     w[1] = r[1] >> 8 | r[2] << 16;
     w[2] = r[2] >> 16 | r[3] << 8;
   } else {
-    constexpr int PER = 32 / BITS;
+    constexpr int PAIRS = 16 / BITS;
 #pragma unroll
     for (int g = 0; g < BITS; ++g) {
       uint32_t v = 0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) v = v * (1u << BITS) + code(PER * g + i); // first code on top
-      w[g] = __byte_perm(v, 0, 0x0123);
+      for (int i = 0; i < PAIRS; ++i) {
+        push_code<P, BITS>(v, u[PAIRS * g + i].x, table, copy);
+        push_code<P, BITS>(v, u[PAIRS * g + i].y, table, copy);
+      }
+      w[g] = __byte_perm(v, 0, 0x0123); // the first code is on top
     }
   }
 }
@@ -132,24 +138,24 @@ template <int BITS> __device__ __forceinline__ void store_words(uint8_t *p, cons
     for (int i = 0; i < 3; ++i) reinterpret_cast<uint32_t *>(p)[i] = w[i];
   }
 }
-// One side of the append: tiles of up to rows_per_block rows, token by token.
+// One side of the append.  A warp takes 32 / (P/32) rows at a time, token by token, and meets no barrier; the turns of its
+// tokens (usually one: the heads of a token are neighbours) go through its own shared memory, cosines and sines apart so
+// that they are read as pairs.
 template <int P, int BITS>
 __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src, long long src_token, long long src_head,
-                                            bool vec, uint8_t *pages, float *scales, bool rotate, float2 *turns,
-                                            TokenPlace *place, uint2 *table) {
-  constexpr int LANES = P / 32;
-  const int heads = a.c.heads, dim = a.c.dim, half = a.r.dim >> 1, ROWS = a.tile_rows;
-  const long long n_rows = a.n_tokens * heads;
-  const int lane = threadIdx.x & 31, part = lane % LANES, d0 = part * 32;
-  if constexpr (BITS != 2) fill_buckets<BITS>(table, threadIdx.x);
-  for (long long r0 = (long long)blockIdx.x * ROWS; r0 < n_rows; r0 += (long long)gridDim.x * ROWS) {
+                                            bool vec, uint8_t *pages, float *scales, bool rotate, float *turns, const uint2 *table) {
+  constexpr int LANES = P / 32, ROWS = rows_per_warp<P>;
+  const int heads = a.c.heads, dim = a.c.dim, half = a.r.dim >> 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % LANES, d0 = part * 32;
+  const uint32_t copy = (lane & (BUCKET_COPIES - 1)) * 8;
+  const long long n_rows = a.n_tokens * heads, stride = (long long)gridDim.x * (ROWS_THREADS / 32) * ROWS;
+  for (long long r0 = ((long long)blockIdx.x * (ROWS_THREADS / 32) + warp) * ROWS; r0 < n_rows; r0 += stride) {
     const long long t0 = r0 / heads;
-    const int in_first = (int)(r0 - t0 * heads); // rows of token t0 before this tile
+    const int in_first = (int)(r0 - t0 * heads); // rows of token t0 before these
     const int live_rows = (int)min((long long)ROWS, n_rows - r0);
     const int nt = (in_first + live_rows - 1) / heads + 1;
-    const int local = min((int)threadIdx.x / LANES, live_rows - 1);
+    const int local = min(lane / LANES, live_rows - 1);
     const int dt = (in_first + local) / heads, h = in_first + local - dt * heads;
-    const bool live = threadIdx.x / LANES < live_rows;
     const long long at = (t0 + dt) * src_token + h * src_head;
 
     float2 x[16];
@@ -172,36 +178,59 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
       }
     }
     const uint32_t signs = a.c.signs[h * LANES + part];
+    // lane i finds the place of token i of these (as many as there are rows at most)
+    TokenPlace mine{-1, 0, 0};
+    if (lane < nt) mine = find_place(a, t0 + lane);
+    const int page = __shfl_sync(0xffffffffu, mine.page, dt), off = __shfl_sync(0xffffffffu, mine.off, dt);
 
-    __syncthreads(); // the previous tile's places and turns have been used
-    find_places<P>(a, t0, nt, place);
-    __syncthreads();
     if (rotate) {
-      for (int i = threadIdx.x; i < nt * half; i += ROWS_THREADS) turns[i] = rotary_turn(a.r, i % half, place[i / half].pos);
-      __syncthreads();
-      const float2 *cs = turns + dt * half;
+      __syncwarp();
+      for (int i = 0; i < nt; ++i) {
+        const long long pos = __shfl_sync(0xffffffffu, mine.pos, i);
+        for (int pair = lane; pair < half; pair += 32) {
+          const float2 k = rotary_turn(a.r, pair, pos);
+          turns[i * 2 * half + pair] = k.x;
+          turns[i * 2 * half + half + pair] = k.y;
+        }
+      }
+      __syncwarp();
+      const float *cs = turns + dt * 2 * half, *sn = cs + half;
       if (a.r.interleaved) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (d0 + 2 * i < a.r.dim) {
-            const float2 k = cs[(d0 >> 1) + i];
+            const float2 k = make_float2(cs[(d0 >> 1) + i], sn[(d0 >> 1) + i]);
             x[i] = make_float2(rotary_first(x[i].x, x[i].y, k), rotary_second(x[i].y, x[i].x, k));
           }
-      } else {
-        // the partner of coordinate i is i +- half: in another lane's same place where half is a
-        // multiple of 32, else fetched again (from L1)
-        const bool shuffle = (half & 31) == 0;
-        const int m = half >> 5, from = (lane & ~(LANES - 1)) + (part < m ? part + m : part < 2 * m ? part - m : part);
+      } else if ((half & 31) == 0) { // the partners of a lane's 32 coordinates are another lane's 32
+        const int m = half >> 5;
+        const bool first = part < m, in = part < 2 * m;
+        const int from = lane + (first ? m : in ? -m : 0);
+        const float sign = first ? -1.f : 1.f;
+        const float *c = cs + (first ? d0 : d0 - half), *s = c + half;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float2 o[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            o[j] = __fmul2_rn(make_float2(__shfl_sync(0xffffffffu, x[i + j].x, from), __shfl_sync(0xffffffffu, x[i + j].y, from)), make_float2(sign, sign));
+          if (in) {
+            const float4 kc = *reinterpret_cast<const float4 *>(c + 2 * i), ks = *reinterpret_cast<const float4 *>(s + 2 * i);
+            // as rotary_first and rotary_second round it
+            x[i] = __ffma2_rn(x[i], make_float2(kc.x, kc.y), __fmul2_rn(o[0], make_float2(ks.x, ks.y)));
+            x[i + 1] = __ffma2_rn(x[i + 1], make_float2(kc.z, kc.w), __fmul2_rn(o[1], make_float2(ks.z, ks.w)));
+          }
+        }
+      } else { // any other: the partner is fetched again (from L1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const int d = d0 + i;
-          const bool first = d < half, in = d < a.r.dim;
-          float &v = (i & 1) ? x[i >> 1].y : x[i >> 1].x;
-          float other = 0.f;
-          if (shuffle) other = __shfl_sync(0xffffffffu, v, from);
-          else if (in) other = load_one(src, at + (first ? d + half : d - half), a.type);
-          if (in) {
-            const float2 k = cs[first ? d : d - half];
+          if (d < a.r.dim) {
+            const bool first = d < half;
+            const int pair = first ? d : d - half;
+            const float2 k = make_float2(cs[pair], sn[pair]);
+            const float other = load_one(src, at + (first ? d + half : pair), a.type);
+            float &v = (i & 1) ? x[i >> 1].y : x[i >> 1].x;
             v = first ? rotary_first(v, other, k) : rotary_second(v, other, k);
           }
         }
@@ -225,26 +254,28 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = __fmul2_rn(x[i], make_float2(inv, inv));
     uint32_t w[BITS];
-    pack_codes<P, BITS>(x, table + (lane & (BUCKET_COPIES - 1)), w);
+    pack_codes<P, BITS>(x, table, copy, w);
 
-    const TokenPlace p = place[dt];
-    if (live && p.page >= 0) {
-      const long long slot = (((long long)p.page * heads + h) << a.c.page_shift) + p.off;
+    if (lane / LANES < live_rows && page >= 0) {
+      const long long slot = (((long long)page * heads + h) << a.c.page_shift) + off;
       store_words<BITS>(pages + slot * (P * BITS / 8) + part * (4 * BITS), w);
       if (part == 0) scales[slot] = norm;
     }
   }
 }
 
-// blockIdx.y: 0 = keys, 1 = values.  Dynamic shared memory: the turns of a tile's tokens.
-template <int P, int KB, int VB> __global__ void __launch_bounds__(ROWS_THREADS) paged_append_kernel(const RowsLaunch a) {
-  extern __shared__ float2 turns[];
-  __shared__ uint2 table[BUCKETS * BUCKET_COPIES];
-  __shared__ TokenPlace place[rows_per_block<P>];
-  if (blockIdx.y == 0)
-    append_rows<P, KB>(a, a.k, a.k_token, a.k_head, a.k_vec, a.c.k_pages, a.c.k_scales, a.r.dim > 0, turns, place, table);
-  else
-    append_rows<P, VB>(a, a.v, a.v_token, a.v_head, a.v_vec, a.c.v_pages, a.c.v_scales, false, turns, place, table);
+// blockIdx.y: 0 = keys, 1 = values.  Dynamic shared memory: the warps' turns.
+template <int P, int KB, int VB> __global__ void __launch_bounds__(ROWS_THREADS, 3) paged_append_kernel(const RowsLaunch a) {
+  extern __shared__ __align__(16) float turns[];
+  __shared__ __align__(128) uint2 table[BUCKETS * BUCKET_COPIES];
+  float *mine = turns + (threadIdx.x >> 5) * a.turn_tokens * a.r.dim;
+  if (blockIdx.y == 0) {
+    if constexpr (KB != 2) { fill_buckets<KB>(table, threadIdx.x); __syncthreads(); }
+    append_rows<P, KB>(a, a.k, a.k_token, a.k_head, a.k_vec, a.c.k_pages, a.c.k_scales, a.r.dim > 0, mine, table);
+  } else {
+    if constexpr (VB != 2) { fill_buckets<VB>(table, threadIdx.x); __syncthreads(); }
+    append_rows<P, VB>(a, a.v, a.v_token, a.v_head, a.v_vec, a.c.v_pages, a.c.v_scales, false, mine, table);
+  }
 }
 
 // Read-back.  A warp takes 16 tokens of one head.  A code becomes the pair {upper, lower} of float16 parts of its
@@ -261,46 +292,61 @@ template <int BITS> __device__ __forceinline__ uint32_t code_bytes(const uint32_
 }
 template <int BITS> __device__ __forceinline__ constexpr int code_byte(int i) { return BITS == 4 ? (i >> 1) & 3 : BITS == 2 ? (i >> 2) & 3 : 3 - ((i >> 1) & 3); }
 
-constexpr int READ_WARPS = 8;
+constexpr int READ_WARPS = 8, READ_TOKENS = 64;
 
 template <int P, int BITS>
-__device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long long dst_token, long long dst_head, bool vec,
+__device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long long dst_token, long long dst_head, int vec,
                                           const uint8_t *pages, const float *scales, uint32_t (*level)[32], TokenPlace *place) {
   constexpr int N = P / 4, S = N / 2, WORDS = (N * BITS / 8 + 3) / 4;
   const int heads = a.c.heads, dim = a.c.dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const long long t0 = (long long)blockIdx.x * 16;
-  const int nt = (int)min(16ll, a.n_tokens - t0);
+  const long long t0 = (long long)blockIdx.x * a.block_tokens;
+  const int nt = (int)min((long long)a.block_tokens, a.n_tokens - t0);
   // a copy of the codebook for every lane: 32 reads of any codes hit 32 banks
   for (int i = threadIdx.x; i < (32 << BITS); i += READ_WARPS * 32) {
     const float c = c_cb[BITS - 2][i >> 5], upper = __half2float(__float2half_rn(c));
     level[i >> 5][i & 31] = pack2(upper, c - upper, TYPE_F16);
   }
-  find_places<P>(a, t0, nt, place);
+  if (threadIdx.x < nt) place[threadIdx.x] = find_place(a, t0 + threadIdx.x);
   __syncthreads();
   const uint32_t mine = smem_u32(&level[0][lane]);
   const int odd = __popc(t & (g >> 1)) & 1;
   const uint32_t b0 = odd ? 0xbc00bc00u : 0x3c003c00u, b1 = odd ^ (g & 1) ? 0xbc00bc00u : 0x3c003c00u; // {1, 1} or {-1, -1}
-  TokenPlace p[2];
+  // items: tiles of 16 tokens, heads; the codes of the next one are on their way while one is worked on
+  const int items = (nt + 15) / 16 * heads, step = gridDim.z * READ_WARPS;
+  uint32_t next[2][WORDS];
+  float norm[2];
+  auto fetch = [&](int item) {
+    const int tile = item / heads, h = item - tile * heads;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) p[r] = g + 8 * r < nt ? place[g + 8 * r] : TokenPlace{-1, 0, 0};
-  for (int h = blockIdx.z * READ_WARPS + warp; h < heads; h += gridDim.z * READ_WARPS) {
+    for (int r = 0; r < 2; ++r) {
+      norm[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) next[r][i] = 0;
+      const int row = 16 * tile + g + 8 * r;
+      if (row < nt && place[row].page >= 0) {
+        const long long slot = (((long long)place[row].page * heads + h) << a.c.page_shift) + place[row].off;
+        load_packed<N * BITS / 8>(pages + slot * (P * BITS / 8) + t * (N * BITS / 8), next[r]);
+        norm[r] = scales[slot];
+      }
+    }
+  };
+  int item = blockIdx.z * READ_WARPS + warp;
+  if (item < items) fetch(item);
+  for (; item < items; item += step) {
+    const int tile = item / heads, h = item - tile * heads;
     uint32_t w[2][WORDS], g24[2][BITS == 3 ? N / 8 : 1];
     float scale[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      scale[r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < WORDS; ++i) w[r][i] = 0;
-      if (p[r].page >= 0) {
-        const long long slot = (((long long)p[r].page * heads + h) << a.c.page_shift) + p[r].off;
-        load_packed<N * BITS / 8>(pages + slot * (P * BITS / 8) + t * (N * BITS / 8), w[r]);
-        scale[r] = scales[slot] * (1.f / P);
-      }
+      for (int i = 0; i < WORDS; ++i) w[r][i] = next[r][i];
+      scale[r] = norm[r] * (1.f / P);
       if constexpr (BITS == 3) {
 #pragma unroll
         for (int i = 0; i < N / 8; ++i) g24[r][i] = spread6(group24<WORDS>(w[r], i));
       }
     }
+    if (item + step < items) fetch(item + step);
     float2 x[2][S]; // coordinates 2s, 2s+1 of this lane's part
 #pragma unroll
     for (int s = 0; s < S; ++s) {
@@ -310,8 +356,8 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           e[r][i] = table_one(__dp4a(code_bytes<BITS>(w[r], 2 * s + i, g24[r]), 0x80u << (8 * code_byte<BITS>(2 * s + i)), mine));
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_16816(d, e[0][0], e[1][0], e[0][1], e[1][1], b0, b1);
+      float d[4];
+      mma_16816_zero(d, e[0][0], e[1][0], e[0][1], e[1][1], b0, b1);
       x[0][s] = make_float2(d[0], d[1]);
       x[1][s] = make_float2(d[2], d[3]);
     }
@@ -340,9 +386,19 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      if (p[r].page < 0) continue;
-      const long long at = (t0 + g + 8 * r) * dst_token + h * dst_head + t * N;
-      if (vec) {
+      const int row = 16 * tile + g + 8 * r;
+      if (row >= nt || place[row].page < 0) continue;
+      const long long at = (t0 + row) * dst_token + h * dst_head + t * N;
+      if (vec == 2 && a.type != TYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 16)
+          if (t * N + i < dim) {
+            uint32_t v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = pack2(x[r][i / 2 + j].x, x[r][i / 2 + j].y, a.type);
+            store_32(static_cast<uint16_t *>(dst) + at + i, v);
+          }
+      } else if (vec) {
 #pragma unroll
         for (int i = 0; i < N; i += 8)
           if (t * N + i < dim) {
@@ -358,10 +414,10 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
   }
 }
 
-// Grid: 16 tokens, side (keys, values), share of the heads.
+// Grid: block_tokens tokens, side (keys, values), share of their items.
 template <int P, int KB, int VB> __global__ void __launch_bounds__(READ_WARPS * 32) paged_read_kernel(const RowsLaunch a) {
   __shared__ uint32_t level[16][32];
-  __shared__ TokenPlace place[16];
+  __shared__ TokenPlace place[READ_TOKENS];
   if (blockIdx.y == 0)
     read_rows<P, KB>(a, a.k, a.k_token, a.k_head, a.k_vec, a.c.k_pages, a.c.k_scales, level, place);
   else

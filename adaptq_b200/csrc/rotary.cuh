@@ -22,7 +22,7 @@ struct RotaryLaunch {
 constexpr int ROTARY_THREADS = 256;
 
 __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaunch a) {
-  extern __shared__ float2 turns[]; // [tokens_per_block][r.dim / 2]
+  extern __shared__ float2 rotary_turns[]; // [tokens_per_block][r.dim / 2]
   const int half = a.r.dim >> 1;
   const long long t0 = (long long)blockIdx.x * a.tokens_per_block;
   const int nt = (int)min((long long)a.tokens_per_block, a.n_tokens - t0);
@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
                                          : (long long)static_cast<const int *>(a.positions)[t0 + t];
     float2 cs = rotary_turn(a.r, pair, pos);
     if (a.inverse) cs.y = -cs.y;
-    turns[i] = cs;
+    rotary_turns[i] = cs;
   }
   __syncthreads();
   if (a.vec) {
@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
     for (int i = threadIdx.x; i < n; i += ROTARY_THREADS) {
       const int part = i % parts, th = i / parts, h = h0 + th % nh, t = th / nh;
       const long long xi = (t0 + t) * a.x_token + h * a.x_head, yi = (t0 + t) * a.y_token + h * a.y_head;
-      const float2 *cs = turns + t * half;
+      const float2 *cs = rotary_turns + t * half;
       float u[8], w[8];
       if (a.r.interleaved) {
         const int d = part << 3;
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
       const long long xi = (t0 + t) * a.x_token + h * a.x_head, yi = (t0 + t) * a.y_token + h * a.y_head;
       if (part < half) {
         const int d = a.r.interleaved ? 2 * part : part, e = a.r.interleaved ? d + 1 : d + half;
-        const float2 k = turns[t * half + part];
+        const float2 k = rotary_turns[t * half + part];
         const float u = load_one(a.x, xi + d, a.type), v = load_one(a.x, xi + e, a.type);
         store_one(a.y, yi + d, a.type, rotary_first(u, v, k));
         store_one(a.y, yi + e, a.type, rotary_second(v, u, k));
