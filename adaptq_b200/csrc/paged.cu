@@ -74,9 +74,10 @@ template <int P, int KB, int VB> void launch_rows(const RowsLaunch &a, bool appe
     constexpr int ROWS = rows_per_warp<P>, WARPS = ROWS_THREADS / 32;
     RowsLaunch b = a;
     b.turn_tokens = std::min(ROWS, (ROWS + a.c.heads - 2) / a.c.heads + 1);
-    const long long passes = (a.n_tokens * a.c.heads + ROWS * WARPS - 1) / (ROWS * WARPS);
-    // a block takes several passes where there are many: its table is filled once
-    const unsigned blocks = (unsigned)std::min(passes, std::max(592ll, (passes + 15) / 16));
+    // several tokens a warp, since what it sets up is paid once, and three rounds of warps (24 an SM, keys and values), for
+    // keys take longer than values
+    b.job_tokens = (int)std::max(1ll, std::min(32ll, 2 * a.n_tokens / (3 * 148 * 24)));
+    const unsigned blocks = (unsigned)((a.n_tokens + b.job_tokens * WARPS - 1) / (b.job_tokens * WARPS));
     paged_append_kernel<P, KB, VB><<<dim3(blocks, 2), ROWS_THREADS, (size_t)WARPS * b.turn_tokens * a.r.dim * sizeof(float), s>>>(b);
   } else {
     RowsLaunch b = a;

@@ -69,8 +69,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int type) {
 }
 
 // Eight consecutive elements; the address is 16-byte aligned.
-__device__ __forceinline__ void load_eight(const void *p, long long i, int type, float *v) {
-  if (type == TYPE_F32) {
+template <int TYPE> __device__ __forceinline__ void load_eight(const void *p, long long i, float *v) {
+  if constexpr (TYPE == TYPE_F32) {
     const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
     const float4 b = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + 4);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -79,19 +79,26 @@ __device__ __forceinline__ void load_eight(const void *p, long long i, int type,
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 f = unpack2(u[j], type);
+      const float2 f = unpack2(u[j], TYPE);
       v[2 * j] = f.x; v[2 * j + 1] = f.y;
     }
   }
 }
-__device__ __forceinline__ void store_eight(void *p, long long i, int type, const float *v) {
-  if (type == TYPE_F32) {
+template <int TYPE> __device__ __forceinline__ void store_eight(void *p, long long i, const float *v) {
+  if constexpr (TYPE == TYPE_F32) {
     *reinterpret_cast<float4 *>(static_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
     *reinterpret_cast<float4 *>(static_cast<float *>(p) + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
   } else {
     *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) =
-        make_uint4(pack2(v[0], v[1], type), pack2(v[2], v[3], type), pack2(v[4], v[5], type), pack2(v[6], v[7], type));
+        make_uint4(pack2(v[0], v[1], TYPE), pack2(v[2], v[3], TYPE), pack2(v[4], v[5], TYPE), pack2(v[6], v[7], TYPE));
   }
+}
+// f(type as a constant): one branch in front of a loop instead of one in it.
+template <int TYPE> struct TypeConstant { static constexpr int value = TYPE; };
+template <typename F> __device__ __forceinline__ void with_type(int type, F f) {
+  if (type == TYPE_BF16) f(TypeConstant<TYPE_BF16>());
+  else if (type == TYPE_F16) f(TypeConstant<TYPE_F16>());
+  else f(TypeConstant<TYPE_F32>());
 }
 
 // Page and place of position `pos` of a sequence whose table row is `row`; false (and a bit

@@ -8,9 +8,9 @@
 // with other warps until it is done.  A run that starts or ends inside an item leaves a partial
 // result; a block joins those of its warps when all are done, and paged_join_kernel those of
 // items that span blocks.
-// Bulk copies were tried first: one costs its SM 80 clocks to issue, whatever its size, and a unit
+// Bulk copies were tried first: issuing one costs its SM 80 clocks, whatever its size, and a unit
 // takes four of them, or sixteen with pages of 16 tokens (33 sequences x 14 heads, 64 coordinates:
-// 60 us against 25).
+// 60 us a call against 39 with everything else equal).
 //
 // Arithmetic.  Codes become float16 values by table look-up: two codes are one index, its
 // entry the two values side by side, and every entry lies in shared memory once per lane, so
@@ -48,7 +48,8 @@ template <int KB, int VB, int P, int MODE> struct AttendShape {
   static constexpr int K_ROW = P * KB / 8, V_ROW = P * VB / 8;
   static constexpr int STAGE = U * (K_ROW + V_ROW + 8);
   static constexpr int COLS = SPLIT ? 4 : 8; // queries of a pass
-  static constexpr int table_bytes(int bits) { return EXACT ? 256 << (2 * bits) : bits == 2 ? 32768 : 128 << (2 * bits); }
+  static constexpr int ROUNDS = EXACT ? 1 : U / 32; // unrolled: EXACT would not fit the instruction cache
+  static constexpr int table_bytes(int bits) { return bits == 2 && !EXACT ? 32768 : 128 << (2 * bits); }
   static constexpr int K_TABLE = 0, V_TABLE = KB == VB ? 0 : table_bytes(KB);
   static constexpr int TABLES = table_bytes(KB) + (KB == VB ? 0 : table_bytes(VB));
   static constexpr int PER_WARP = 2 * STAGE + 48;
@@ -99,18 +100,19 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) { return pack2(
 
 // Tables.  BITS bits a code; the index is (first code << BITS) | second code.
 //   narrow, one part:   4 bytes {first, second} x 32 lanes
-//   narrow, two parts:  8 bytes {first, second upper; first, second lower} x 32 lanes
+//   narrow, two parts:  8 bytes {first, second upper; first, second lower} x 16 lanes (a 64-bit read serves half a warp
+//                       at a time)
 //   wide (2 bits):      index = 4 codes of a byte, 8 bytes x 16 lanes
 template <int BITS, bool EXACT> __device__ __forceinline__ void fill_table(uint8_t *table, int tid, int threads) {
   const float *c = c_cb[BITS - 2];
   constexpr float F = table_scale(BITS);
   if constexpr (EXACT) {
-    for (int i = tid; i < (32 << (2 * BITS)); i += threads) {
-      const int index = i >> 5;
-      const float a = c[index >> BITS] * F, b = c[index & ((1 << BITS) - 1)] * F;
-      const float ah = __half2float(__float2half_rn(a)), bh = __half2float(__float2half_rn(b));
-      // the lower part from the unrounded product
-      reinterpret_cast<uint2 *>(table)[i] = make_uint2(half2_bits(a, b), half2_bits(fmaf(c[index >> BITS], F, -ah), fmaf(c[index & ((1 << BITS) - 1)], F, -bh)));
+    for (int i = tid; i < (16 << (2 * BITS)); i += threads) {
+      const int index = i >> 4;
+      const float a = c[index >> BITS], b = c[index & ((1 << BITS) - 1)];
+      const uint32_t upper = half2_bits(a * F, b * F);
+      const float2 u = unpack2(upper, TYPE_F16);
+      reinterpret_cast<uint2 *>(table)[i] = make_uint2(upper, half2_bits(fmaf(a, F, -u.x), fmaf(b, F, -u.y))); // from the unrounded products
     }
   } else if constexpr (BITS == 2) {
     for (int i = tid; i < 256 * 16; i += threads) {
@@ -178,8 +180,8 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
     // Tokens are assigned to rows so that neither the reads of key rows (rows g, g+8) nor those of value
     // rows (rows 2t, 2t+1, 2t+8, 2t+9) of 32 or 64 bytes meet in a bank more often than their size makes them.
     phi = (g & 1) ? 7 - (g >> 1) : g >> 1;
-    k_table = smem_u32(attend_smem) + S::K_TABLE + (EXACT ? ln * 8 : KB == 2 ? (ln & 15) * 8 : ln * 4);
-    v_table = smem_u32(attend_smem) + S::V_TABLE + (EXACT ? ln * 8 : VB == 2 ? (ln & 15) * 8 : ln * 4);
+    k_table = smem_u32(attend_smem) + S::K_TABLE + (EXACT || KB == 2 ? (ln & 15) * 8 : ln * 4);
+    v_table = smem_u32(attend_smem) + S::V_TABLE + (EXACT || VB == 2 ? (ln & 15) * 8 : ln * 4);
   }
 
   // Codes 2p, 2p+1 of this lane's part of a key row.
@@ -206,7 +208,7 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
     const uint8_t *keys = attend_smem + stage, *vals = keys + U * S::K_ROW;
     const float *ks = reinterpret_cast<const float *>(attend_smem + stage + U * (S::K_ROW + S::V_ROW)), *vs = ks + U;
     float s[TILES][4];
-#pragma unroll
+#pragma unroll (EXACT ? 1 : TILES / 2)
     for (int round = 0; round < TILES / 2; ++round) {
 #pragma unroll
     for (int i = 0; i + 2 < TILES; ++i) {
@@ -238,6 +240,7 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
           }
         }
       } else {
+        float odd[4] = {}, low[4] = {}; // EXACT
 #pragma unroll
         for (int k = 0; k < DIM_TILES; ++k) {
           uint32_t word[2][2];
@@ -251,9 +254,11 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
-              for (int p = 0; p < 2; ++p) v[r][p] = table_two(entry_address<2 * KB, 8>(k_table, word[r][p], pos[p]));
-            mma_16816(s[i], v[0][0].x, v[1][0].x, v[0][1].x, v[1][1].x, qb[2 * k], qb[2 * k + 1]);
-            mma_16816(s[i], v[0][0].y, v[1][0].y, v[0][1].y, v[1][1].y, qb[2 * k], qb[2 * k + 1]);
+              for (int p = 0; p < 2; ++p) v[r][p] = table_two(entry_address<2 * KB, 7>(k_table, word[r][p], pos[p]));
+            // The tensor cores cut sums off instead of rounding them: short chains, added up in float32.
+            if (k & 1) mma_16816(odd, v[0][0].x, v[1][0].x, v[0][1].x, v[1][1].x, qb[2 * k], qb[2 * k + 1]);
+            else mma_16816(s[i], v[0][0].x, v[1][0].x, v[0][1].x, v[1][1].x, qb[2 * k], qb[2 * k + 1]);
+            mma_16816(low, v[0][0].y, v[1][0].y, v[0][1].y, v[1][1].y, qb[2 * k], qb[2 * k + 1]);
           } else {
             uint32_t v[2][2];
 #pragma unroll
@@ -262,6 +267,10 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
               for (int p = 0; p < 2; ++p) v[r][p] = table_one(entry_address<2 * KB, 7>(k_table, word[r][p], pos[p]));
             mma_16816(s[i], v[0][0], v[1][0], v[0][1], v[1][1], qb[2 * k], qb[2 * k + 1]);
           }
+        }
+        if constexpr (EXACT) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] += odd[j] + low[j];
         }
       }
     }
@@ -328,7 +337,7 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
           l[e] += p;
           z = p * norm[i][r];
         }
-#pragma unroll
+#pragma unroll (EXACT ? 1 : TILES / 2)
     for (int round = 0; round < TILES / 2; ++round) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -385,7 +394,7 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
           if constexpr (EXACT) {
             uint2 v[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = table_two(entry_address<2 * VB, 8>(v_table, src[q], pos));
+            for (int q = 0; q < 4; ++q) v[q] = table_two(entry_address<2 * VB, 7>(v_table, src[q], pos));
             mma_16816(acc[j], v[0].x, v[1].x, v[2].x, v[3].x, wt[0], wt[1]);
             mma_16816(acc[j], v[0].y, v[1].y, v[2].y, v[3].y, wt[0], wt[1]);
           } else {
@@ -559,38 +568,39 @@ template <typename S> struct AttendWalk {
     b = h = pass = u = len = page = 0;
     nu = 1;
     const int per_seq = a.c.heads * a.passes;
-    // units before every lane's share of the sequences
+    // units before every lane's share of the sequences (the host refuses calls whose units 31 bits would not count)
     const int chunk = (a.n_seqs + 31) / 32, b0 = min(a.n_seqs, lane * chunk), b1 = min(a.n_seqs, b0 + chunk);
-    long long sum = 0;
+    int sum = 0;
 #pragma unroll 4
     for (int i = b0; i < b1; ++i) sum += (clipped_length(a, i, blockIdx.x == 0 && warp == 0) + U - 1) / U;
     sum *= per_seq;
-    const long long own = sum;
+    const int own = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += v;
     }
-    const long long total = __shfl_sync(0xffffffffu, sum, 31), before = sum - own;
+    const int total = __shfl_sync(0xffffffffu, sum, 31), before = sum - own;
     // blocks share the units evenly, and so do the warps of a block; no block is without any as long as there are some
-    const int blocks = (int)min((long long)gridDim.x, total);
-    if ((int)blockIdx.x >= blocks) return 0;
-    const long long first = total * blockIdx.x / blocks;
-    const int share = (int)(total * (blockIdx.x + 1) / blocks - first);
-    const int skip = (int)((long long)share * warp / S::WARPS), units = (int)((long long)share * (warp + 1) / S::WARPS) - skip;
+    const int blocks = min((int)gridDim.x, total), block = blockIdx.x;
+    if (block >= blocks) return 0;
+    const int even = total / blocks, more = total - even * blocks;
+    const int first = even * block + min(block, more), share = even + (block < more);
+    const int per_warp = share / S::WARPS, rest_warps = share - per_warp * S::WARPS;
+    const int units = per_warp + (warp < rest_warps);
     if (units == 0) return 0;
     // the last lane whose share begins at or before the run, then along that share
-    long long rest = first + skip;
+    int rest = first + per_warp * warp + min(warp, rest_warps);
     const int at = 31 - __clz(__ballot_sync(0xffffffffu, before <= rest));
     rest -= __shfl_sync(0xffffffffu, before, at);
     for (b = at * chunk;; ++b) {
       len = clipped_length(a, b, false);
       nu = (len + U - 1) / U;
-      if (rest < (long long)nu * per_seq) break;
-      rest -= (long long)nu * per_seq;
+      if (rest < nu * per_seq) break;
+      rest -= nu * per_seq;
     }
-    const int hp = (int)(rest / nu);
-    u = (int)(rest - (long long)hp * nu);
+    const int hp = rest / nu;
+    u = rest - hp * nu;
     h = hp / a.passes;
     pass = hp - h * a.passes;
     find_pages(a);
@@ -628,7 +638,9 @@ template <typename S> struct AttendWalk {
           const int per = a.c.page_size, at = p << a.c.page_shift;
           const long long row = ((long long)__shfl_sync(0xffffffffu, page, p) * a.c.heads + h) << a.c.page_shift;
           const uint8_t *k = a.c.k_pages + row * S::K_ROW, *v = a.c.v_pages + row * S::V_ROW;
+#pragma unroll 1
           for (int i = lane * 16; i < per * S::K_ROW; i += 512) copy_16(to + at * S::K_ROW + i - lane * 16, k + i);
+#pragma unroll 1
           for (int i = lane * 16; i < per * S::V_ROW; i += 512) copy_16(to + U * S::K_ROW + at * S::V_ROW + i - lane * 16, v + i);
           if (norm_at < per * 4 && lane * 16 < 8 * U) copy_16(to + U * (S::K_ROW + S::V_ROW) + at * 4, norms + row * 4 + norm_at);
         }

@@ -22,7 +22,8 @@ struct RowsLaunch {
   // the model's rows: keys and values (read by the append, written by the read-back)
   void *k, *v;
   long long k_token, k_head, v_token, v_head;
-  int turn_tokens;        // append: tokens of a warp's rows at most
+  int job_tokens;         // append: tokens of a warp, at most 32
+  int turn_tokens;        // append: tokens of a warp's rows in hand at most
   int block_tokens;       // read-back: tokens of a block
   int type, k_vec, v_vec; // 0; 1: rows 16-byte aligned, dim a multiple of 8; 2: 32-byte aligned, a multiple of 16 as well
 };
@@ -68,7 +69,7 @@ template <int P> __device__ __forceinline__ void row_butterflies(float2 (&x)[16]
   }
 }
 
-// Quantiser of 3 and 4 bits: the 128 buckets of a quarter from -16 on hold at most one threshold each, so a code is the
+// Quantisers.  2 bits: evenly spaced thresholds, one rounding.  3 and 4 bits: the 128 buckets of a quarter from -16 on hold at most one threshold each, so a code is the
 // count of thresholds at or below the bucket's start and one comparison.  16 copies of the table, entry by entry, keep the
 // half-warps of a 64-bit read apart.  A coordinate is at most sqrt(P) = 16 in size.
 constexpr int BUCKETS = 128, BUCKET_COPIES = 16;
@@ -87,8 +88,12 @@ template <int BITS> __device__ __forceinline__ void fill_buckets(uint2 *table, i
 }
 // word = word << BITS | code of u
 template <int P, int BITS> __device__ __forceinline__ void push_code(uint32_t &word, float u, const uint2 *table, uint32_t copy /* 8 * lane's copy */) {
-  if constexpr (BITS == 2) word = word * 4 + (uint32_t)quantize_value<2>(u);
-  else {
+  if constexpr (BITS == 2) {
+    // thresholds -T, 0, T: the code is floor(u / T) + 2 within 0 .. 3
+    constexpr float T = (0.4528f + 1.5104f) * 0.5f;
+    const float v = fminf(fmaxf(u, -1.5f * T), 1.5f * T);
+    word = word * 4 + (__float_as_uint(__fmaf_rd(v, 1.f / T, 8388608.f + 2.f)) & 3u);
+  } else {
     if constexpr (P == 256) u = fminf(fmaxf(u, -16.f), 15.75f);
     // 4 u + 64 in units of 2^-7, rounded down: the bucket lies where a byte offset into the table wants it (any for NaN)
     const uint32_t at = (__float_as_uint(__fmaf_rd(u, 4.f, 65536.f + 64.f)) & ((BUCKETS - 1) << 7)) | copy;
@@ -148,29 +153,30 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
   const int heads = a.c.heads, dim = a.c.dim, half = a.r.dim >> 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % LANES, d0 = part * 32;
   const uint32_t copy = (lane & (BUCKET_COPIES - 1)) * 8;
-  const long long n_rows = a.n_tokens * heads, stride = (long long)gridDim.x * (ROWS_THREADS / 32) * ROWS;
-  for (long long r0 = ((long long)blockIdx.x * (ROWS_THREADS / 32) + warp) * ROWS; r0 < n_rows; r0 += stride) {
-    const long long t0 = r0 / heads;
-    const int in_first = (int)(r0 - t0 * heads); // rows of token t0 before these
-    const int live_rows = (int)min((long long)ROWS, n_rows - r0);
-    const int nt = (in_first + live_rows - 1) / heads + 1;
-    const int local = min(lane / LANES, live_rows - 1);
-    const int dt = (in_first + local) / heads, h = in_first + local - dt * heads;
+  // a job: the rows of a.job_tokens tokens; lane i finds the place of the i-th
+  const long long t0 = ((long long)blockIdx.x * (ROWS_THREADS / 32) + warp) * a.job_tokens;
+  if (t0 >= a.n_tokens) return;
+  const int tokens = (int)min((long long)a.job_tokens, a.n_tokens - t0), n_rows = tokens * heads;
+  TokenPlace mine{-1, 0, 0};
+  if (lane < tokens) mine = find_place(a, t0 + lane);
+  for (int r0 = 0; r0 < n_rows; r0 += ROWS) {
+    const int row = min(r0 + lane / LANES, n_rows - 1), dt = row / heads, h = row - dt * heads;
+    const int first_token = r0 / heads, nt = min(r0 + ROWS - 1, n_rows - 1) / heads - first_token + 1;
     const long long at = (t0 + dt) * src_token + h * src_head;
 
     float2 x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = make_float2(0.f, 0.f);
-    if (vec) {
+    if (vec) with_type(a.type, [&](auto type) {
 #pragma unroll
       for (int i = 0; i < 32; i += 8)
         if (d0 + i < dim) {
           float v[8];
-          load_eight(src, at + d0 + i, a.type, v);
+          load_eight<decltype(type)::value>(src, at + d0 + i, v);
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[i / 2 + j] = make_float2(v[2 * j], v[2 * j + 1]);
         }
-    } else {
+    }); else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         if (d0 + 2 * i < dim) x[i].x = load_one(src, at + d0 + 2 * i, a.type);
@@ -178,15 +184,12 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
       }
     }
     const uint32_t signs = a.c.signs[h * LANES + part];
-    // lane i finds the place of token i of these (as many as there are rows at most)
-    TokenPlace mine{-1, 0, 0};
-    if (lane < nt) mine = find_place(a, t0 + lane);
     const int page = __shfl_sync(0xffffffffu, mine.page, dt), off = __shfl_sync(0xffffffffu, mine.off, dt);
 
     if (rotate) {
       __syncwarp();
       for (int i = 0; i < nt; ++i) {
-        const long long pos = __shfl_sync(0xffffffffu, mine.pos, i);
+        const long long pos = __shfl_sync(0xffffffffu, mine.pos, first_token + i);
         for (int pair = lane; pair < half; pair += 32) {
           const float2 k = rotary_turn(a.r, pair, pos);
           turns[i * 2 * half + pair] = k.x;
@@ -194,7 +197,7 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
         }
       }
       __syncwarp();
-      const float *cs = turns + dt * 2 * half, *sn = cs + half;
+      const float *cs = turns + (dt - first_token) * 2 * half, *sn = cs + half;
       if (a.r.interleaved) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -256,7 +259,7 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
     uint32_t w[BITS];
     pack_codes<P, BITS>(x, table, copy, w);
 
-    if (lane / LANES < live_rows && page >= 0) {
+    if (r0 + lane / LANES < n_rows && page >= 0) {
       const long long slot = (((long long)page * heads + h) << a.c.page_shift) + off;
       store_words<BITS>(pages + slot * (P * BITS / 8) + part * (4 * BITS), w);
       if (part == 0) scales[slot] = norm;
@@ -389,23 +392,26 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
       const int row = 16 * tile + g + 8 * r;
       if (row >= nt || place[row].page < 0) continue;
       const long long at = (t0 + row) * dst_token + h * dst_head + t * N;
-      if (vec == 2 && a.type != TYPE_F32) {
+      if (vec) with_type(a.type, [&](auto type) {
+        constexpr int TYPE = decltype(type)::value;
+        if (TYPE != TYPE_F32 && vec == 2) {
 #pragma unroll
-        for (int i = 0; i < N; i += 16)
-          if (t * N + i < dim) {
-            uint32_t v[8];
+          for (int i = 0; i < N; i += 16)
+            if (t * N + i < dim) {
+              uint32_t v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = pack2(x[r][i / 2 + j].x, x[r][i / 2 + j].y, a.type);
-            store_32(static_cast<uint16_t *>(dst) + at + i, v);
-          }
-      } else if (vec) {
+              for (int j = 0; j < 8; ++j) v[j] = pack2(x[r][i / 2 + j].x, x[r][i / 2 + j].y, TYPE);
+              store_32(static_cast<uint16_t *>(dst) + at + i, v);
+            }
+        } else {
 #pragma unroll
-        for (int i = 0; i < N; i += 8)
-          if (t * N + i < dim) {
-            const float v[8] = {x[r][i / 2].x, x[r][i / 2].y, x[r][i / 2 + 1].x, x[r][i / 2 + 1].y, x[r][i / 2 + 2].x, x[r][i / 2 + 2].y, x[r][i / 2 + 3].x, x[r][i / 2 + 3].y};
-            store_eight(dst, at + i, a.type, v);
-          }
-      } else {
+          for (int i = 0; i < N; i += 8)
+            if (t * N + i < dim) {
+              const float v[8] = {x[r][i / 2].x, x[r][i / 2].y, x[r][i / 2 + 1].x, x[r][i / 2 + 1].y, x[r][i / 2 + 2].x, x[r][i / 2 + 2].y, x[r][i / 2 + 3].x, x[r][i / 2 + 3].y};
+              store_eight<TYPE>(dst, at + i, v);
+            }
+        }
+      }); else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
           if (t * N + i < dim) store_one(dst, at + i, a.type, (i & 1) ? x[r][i >> 1].y : x[r][i >> 1].x);

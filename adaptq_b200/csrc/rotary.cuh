@@ -36,7 +36,8 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
     rotary_turns[i] = cs;
   }
   __syncthreads();
-  if (a.vec) {
+  if (a.vec) with_type(a.type, [&](auto type) {
+    constexpr int TYPE = decltype(type)::value;
     // one thread: eight neighbours and, in the half layout, their eight partners
     const int parts = a.r.interleaved ? a.dim >> 3 : (a.dim - half) >> 3;
     const int n = nt * nh * parts;
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
       float u[8], w[8];
       if (a.r.interleaved) {
         const int d = part << 3;
-        load_eight(a.x, xi + d, a.type, u);
+        load_eight<TYPE>(a.x, xi + d, u);
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           const bool in = d + j < a.r.dim;
@@ -55,27 +56,27 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
           w[j] = in ? rotary_first(u[j], u[j + 1], k) : u[j];
           w[j + 1] = in ? rotary_second(u[j + 1], u[j], k) : u[j + 1];
         }
-        store_eight(a.y, yi + d, a.type, w);
+        store_eight<TYPE>(a.y, yi + d, w);
       } else if ((part << 3) < half) {
         const int d = part << 3;
         float v[8], z[8];
-        load_eight(a.x, xi + d, a.type, u);
-        load_eight(a.x, xi + d + half, a.type, v);
+        load_eight<TYPE>(a.x, xi + d, u);
+        load_eight<TYPE>(a.x, xi + d + half, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float2 k = cs[d + j];
           w[j] = rotary_first(u[j], v[j], k);
           z[j] = rotary_second(v[j], u[j], k);
         }
-        store_eight(a.y, yi + d, a.type, w);
-        store_eight(a.y, yi + d + half, a.type, z);
+        store_eight<TYPE>(a.y, yi + d, w);
+        store_eight<TYPE>(a.y, yi + d + half, z);
       } else { // behind the rotated part
         const int d = half + (part << 3);
-        load_eight(a.x, xi + d, a.type, u);
-        store_eight(a.y, yi + d, a.type, u);
+        load_eight<TYPE>(a.x, xi + d, u);
+        store_eight<TYPE>(a.y, yi + d, u);
       }
     }
-  } else {
+  }); else {
     // one thread: one pair, or one element behind the rotated part
     const int parts = a.dim - half, n = nt * nh * parts;
     for (int i = threadIdx.x; i < n; i += ROTARY_THREADS) {
