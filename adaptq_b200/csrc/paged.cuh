@@ -111,14 +111,19 @@ __device__ __forceinline__ bool find_slot(const PagedView &c, const int *row, in
   return true;
 }
 
-// The sequence of token t: the last b with cu[b] <= t, if t lies before cu[b+1].
-__device__ __forceinline__ int owner_of(const int *cu, int n_seqs, long long t) {
-  int lo = 0, hi = n_seqs; // cu[lo] <= t wanted, cu[hi] > t wanted
-  if (cu[0] > t || cu[n_seqs] <= t) return -1;
+// The sequence of token t + lane for the whole warp: the last b with cu[b] <= it, or -1 if it lies before the first or
+// behind the last.  The warp searches together for token t, 32 probes a step; the others follow from there.
+__device__ __forceinline__ int owner_of(const int *cu, int n_seqs, long long t, int lane, int count) {
+  int lo = 0, hi = n_seqs; // cu[lo] <= t < cu[hi] if any
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid;
+    const int step = (hi - lo + 31) >> 5, at = lo + (lane + 1) * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at < hi && cu[at] <= t);
+    const int n = __popc(below);
+    hi = min(hi, lo + (n + 1) * step);
+    lo += n * step;
   }
+  if (lane >= count || cu[0] > t + lane || cu[n_seqs] <= t + lane) return -1;
+  while (lo + 1 < n_seqs && cu[lo + 1] <= t + lane) ++lo;
   return lo;
 }
 

@@ -51,7 +51,7 @@ template <typename S> static bool launch_attend(const AttendCall &call) {
   }
   // no more blocks than the tables have room for units
   const long long most = items * ((((long long)a.table.width << a.c.page_shift) + S::U - 1) / S::U);
-  if (most > 0x7fffffff) { aq_set_error("%s: the block tables have room for too many tokens for one call", fn); return false; }
+  if (most > 0x7fffffff || ((long long)a.table.width << a.c.page_shift) > 0x3fffffff) { aq_set_error("%s: the block tables have room for too many tokens for one call", fn); return false; }
   const int blocks = (int)std::max<long long>(1, std::min<long long>(sms, most));
   uint8_t *base = static_cast<uint8_t *>(call.workspace);
   a.operands = reinterpret_cast<uint32_t *>(base);

@@ -30,12 +30,12 @@ struct RowsLaunch {
 
 struct TokenPlace { int page, off; long long pos; }; // page < 0: nowhere
 
-// Where token t goes to, or is read from.
-__device__ __forceinline__ TokenPlace find_place(const RowsLaunch &a, long long t) {
-  const int b = a.cu ? owner_of(a.cu, a.n_seqs, t) : (t < a.n_seqs ? (int)t : -1);
+// Where token t + lane goes to, or is read from, for lanes below `count` (the whole warp calls).
+__device__ __forceinline__ TokenPlace find_place(const RowsLaunch &a, long long t, int lane, int count) {
+  const int b = a.cu ? owner_of(a.cu, a.n_seqs, t, lane, count) : (lane < count && t + lane < a.n_seqs ? (int)t + lane : -1);
   TokenPlace p{-1, 0, 0};
   if (b >= 0 && !(a.start_bias < 0 && a.starts[b] == 0)) { // a decode step leaves empty sequences out
-    p.pos = (long long)a.starts[b] + a.start_bias + (a.cu ? t - a.cu[b] : 0);
+    p.pos = (long long)a.starts[b] + a.start_bias + (a.cu ? t + lane - a.cu[b] : 0);
     if (!find_slot(a.c, a.table.entries + b * a.table.stride, a.table.width, p.pos, p.page, p.off)) p.page = -1;
   }
   return p;
@@ -157,8 +157,7 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
   const long long t0 = ((long long)blockIdx.x * (ROWS_THREADS / 32) + warp) * a.job_tokens;
   if (t0 >= a.n_tokens) return;
   const int tokens = (int)min((long long)a.job_tokens, a.n_tokens - t0), n_rows = tokens * heads;
-  TokenPlace mine{-1, 0, 0};
-  if (lane < tokens) mine = find_place(a, t0 + lane);
+  const TokenPlace mine = find_place(a, t0, lane, tokens);
   for (int r0 = 0; r0 < n_rows; r0 += ROWS) {
     const int row = min(r0 + lane / LANES, n_rows - 1), dt = row / heads, h = row - dt * heads;
     const int first_token = r0 / heads, nt = min(r0 + ROWS - 1, n_rows - 1) / heads - first_token + 1;
@@ -309,7 +308,10 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
     const float c = c_cb[BITS - 2][i >> 5], upper = __half2float(__float2half_rn(c));
     level[i >> 5][i & 31] = pack2(upper, c - upper, TYPE_F16);
   }
-  if (threadIdx.x < nt) place[threadIdx.x] = find_place(a, t0 + threadIdx.x);
+  if (warp * 32 < nt) {
+    const TokenPlace p = find_place(a, t0 + warp * 32, lane, min(32, nt - warp * 32));
+    if (warp * 32 + lane < nt) place[warp * 32 + lane] = p;
+  }
   __syncthreads();
   const uint32_t mine = smem_u32(&level[0][lane]);
   const int odd = __popc(t & (g >> 1)) & 1;

@@ -10,10 +10,11 @@ from __future__ import annotations
 
 import ctypes as C
 
+import numpy as np
 import torch
 
 from . import _lib
-from .rotary import TYPES, Rotary
+from .rotary import TYPES, Rotary, current_stream
 
 _STATUS = ((1, "a block table names a page outside the pool"), (2, "a position or length has no room in its block table"),
            (4, "a kernel gave up waiting for a copy"))
@@ -77,18 +78,17 @@ class PagedKVCache:
         self.n_pages, self.n_kv_heads, self.page_size = (int(s) for s in k_pages.shape[:3])
         self.dim, self.padded, self.k_bits, self.v_bits = int(dim), _padded(dim), int(k_bits), int(v_bits)
         self.device = k_pages.device
+        self._index = self.device.index
         words = self.padded // 32
         if signs is None:
             host = torch.zeros(self.n_kv_heads, words, dtype=torch.int32)
             if self._L.adaptq_paged_signs(C.c_uint64(int(seed) & (2**64 - 1)), self.n_kv_heads, self.dim, host.data_ptr()):
                 raise RuntimeError(_lib.last_error())
         else:
-            s = torch.as_tensor(signs).cpu().to(torch.int64)
-            if tuple(s.shape) != (self.n_kv_heads, self.padded) or not bool((s.abs() == 1).all()):
+            s = torch.as_tensor(signs).cpu().numpy()
+            if s.shape != (self.n_kv_heads, self.padded) or not (np.abs(s) == 1).all():
                 raise ValueError(f"signs must be ({self.n_kv_heads}, {self.padded}) of +1 and -1")
-            bits = (s < 0).to(torch.int64).view(self.n_kv_heads, words, 32) << torch.arange(32)
-            w = bits.sum(-1)
-            host = torch.where(w >= 2**31, w - 2**32, w).to(torch.int32)
+            host = torch.from_numpy(np.packbits(s < 0, axis=1, bitorder="little").view(np.int32))
         self._signs = host.to(self.device)
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._desc = _lib.Paged(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
@@ -96,32 +96,30 @@ class PagedKVCache:
                                 self.dim, self.k_bits, self.v_bits, self.device.index)
         self._ref = C.addressof(self._desc)
         self._scale = self.dim ** -0.5
+        self._sizes = {}  # bytes of attend's workspace by (sequences, query heads, type)
 
     # -- arguments ------------------------------------------------------------------------
     def _ints(self, name, t, n):
-        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 1 or (n is not None and t.shape[0] != n):
-            raise ValueError(f"{name} must be ({'n' if n is None else n},) int32 on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        if t.dtype is not torch.int32 or t.dim() != 1 or len(t) != n or t.get_device() != self._index:
+            raise ValueError(f"{name} must be ({n},) int32 on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
         return t if t.is_contiguous() else t.contiguous()
 
     def _table(self, t):
-        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 2:
-            raise ValueError(f"block_table must be (sequences, pages) int32 on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+        if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[1] == 0 or t.get_device() != self._index:
+            raise ValueError(f"block_table must be (sequences, pages > 0) int32 on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        return t if t.is_contiguous() or t.stride(1) == 1 else t.contiguous()
 
     def _rows(self, name, t, heads):
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.dim or t.dtype not in TYPES or t.device != self.device:
+        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.dim or t.dtype not in TYPES or t.get_device() != self._index:
             raise ValueError(f"{name} must be (n, {heads}, {self.dim}) float32, float16 or bfloat16 on {self.device}, got {tuple(t.shape)} "
                              f"{t.dtype} on {t.device}")
 
     def _rotary(self, rotary):
         if rotary is None:
             return None
-        if not isinstance(rotary, Rotary) or rotary.device != self.device or rotary.dim > self.dim:
+        if not isinstance(rotary, Rotary) or rotary._index != self._index or rotary.dim > self.dim:
             raise ValueError(f"rotary must be a Rotary of at most {self.dim} coordinates on {self.device}")
         return rotary._ref
-
-    def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
 
     # -- operators ------------------------------------------------------------------------
     def append(self, k, v, block_table, starts, cu_tokens=None, rotary=None):
@@ -149,14 +147,14 @@ class PagedKVCache:
         ks, vs = k.stride(), v.stride()
         if self._L.adaptq_paged_append(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], TYPES[k.dtype], table.data_ptr(),
                                        table.stride(0), table.shape[1], starts.data_ptr(), bias,
-                                       None if cu_tokens is None else cu_tokens.data_ptr(), n_seqs, n, self._rotary(rotary), self._stream()):
+                                       None if cu_tokens is None else cu_tokens.data_ptr(), n_seqs, n, self._rotary(rotary), current_stream(self._index)):
             raise RuntimeError(_lib.last_error())
 
     def attend(self, q, block_table, lengths, rotary=None, scale=None, out=None):
         """Attention of one token per sequence over its first lengths[b] tokens.  q: (sequences, query heads, dim), query head
         j reading KV head j // (query heads / KV heads) -> the same shape and type.  Queries are rotated by position
         lengths[b] - 1 first, if `rotary`.  scale: 1/sqrt(dim) by default.  A sequence of length 0 gives zeros."""
-        if q.dim() != 3 or q.shape[2] != self.dim or q.shape[1] % self.n_kv_heads or not q.shape[1] or q.dtype not in TYPES or q.device != self.device:
+        if q.dim() != 3 or q.shape[2] != self.dim or q.shape[1] % self.n_kv_heads or not q.shape[1] or q.dtype not in TYPES or q.get_device() != self._index:
             raise ValueError(f"q must be (sequences, a multiple of {self.n_kv_heads} heads, {self.dim}) float32, float16 or bfloat16 on {self.device}, "
                              f"got {tuple(q.shape)} {q.dtype} on {q.device}")
         q = q if q.stride(2) == 1 else q.contiguous()
@@ -166,18 +164,20 @@ class PagedKVCache:
             raise ValueError(f"block_table has {table.shape[0]} sequences, q {n}")
         lengths = self._ints("lengths", lengths, n)
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = torch.empty((n, heads, self.dim), dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
             raise ValueError("out must have the shape, type and device of q and contiguous rows")
         kind = TYPES[q.dtype]
-        size = self._L.adaptq_paged_attend_workspace(self._ref, n, heads, kind)
+        size = self._sizes.get((n, heads, kind))
+        if size is None:
+            size = self._sizes[n, heads, kind] = self._L.adaptq_paged_attend_workspace(self._ref, n, heads, kind)
         # of this call alone: the allocator hands it on in the order of the stream, also inside a captured graph
         workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
         qs, os = q.stride(), out.stride()
         if self._L.adaptq_paged_attend(self._ref, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], kind, table.data_ptr(),
                                        table.stride(0), table.shape[1], lengths.data_ptr(), n, heads,
                                        self._scale if scale is None else float(scale), self._rotary(rotary), workspace.data_ptr(), size,
-                                       self._stream()):
+                                       current_stream(self._index)):
             raise RuntimeError(_lib.last_error())
         return out
 
@@ -207,7 +207,7 @@ class PagedKVCache:
                 raise ValueError(f"out must be two tensors of {total} rows, of one type, with contiguous rows")
         ks, vs = k.stride(), v.stride()
         if self._L.adaptq_paged_read(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], TYPES[k.dtype], table.data_ptr(),
-                                     table.stride(0), table.shape[1], starts.data_ptr(), cu_tokens.data_ptr(), n_seqs, int(total), self._stream()):
+                                     table.stride(0), table.shape[1], starts.data_ptr(), cu_tokens.data_ptr(), n_seqs, int(total), current_stream(self._index)):
             raise RuntimeError(_lib.last_error())
         return k, v
 

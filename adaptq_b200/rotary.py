@@ -8,12 +8,18 @@ from __future__ import annotations
 import ctypes as C
 import math
 
+import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+try:  # the handle of the current stream without a Stream object around it: 2 us less per call
+    current_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:
+    def current_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
 
 
 def _inverse_frequencies(dim, base, scaling):
@@ -93,9 +99,10 @@ class Rotary:
         if device.type != "cuda":
             raise ValueError(f"Rotary needs a CUDA device, got {device}")
         self._L = _lib.load()
-        turns = [int(w / (2 * math.pi) * 2.0 ** 64) % 2 ** 64 for w in self.inv_freq.tolist()]
-        self._turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
+        turns = ((self.inv_freq.numpy() / (2 * math.pi)) % 1.0 * 2.0 ** 64).astype(np.uint64)
+        self._turns = torch.from_numpy(turns.view(np.int64)).to(device)
         self.device = self._turns.device
+        self._index = self.device.index
         self._desc = _lib.RotaryDesc(self._turns.data_ptr(), self.factor, self.dim, int(self.interleaved))
         self._ref = C.addressof(self._desc)
 
@@ -110,39 +117,44 @@ class Rotary:
         return self._apply(x.detach(), positions, out, 0)
 
     def _apply(self, x, positions, out, inverse):
-        if x.dim() != 3 or x.dtype not in TYPES or x.device != self.device:
+        kind = TYPES.get(x.dtype)
+        if x.dim() != 3 or kind is None or x.get_device() != self._index:
             raise ValueError(f"x must be (tokens, heads, dim) float32, float16 or bfloat16 on {self.device}, got {tuple(x.shape)} "
                              f"{x.dtype} on {x.device}")
         n, heads, dim = x.shape
         if dim < self.dim:
             raise ValueError(f"x has {dim} coordinates a head, the rotation {self.dim}")
-        if positions.shape != (n,) or positions.dtype not in (torch.int32, torch.int64) or positions.device != self.device:
+        wide = positions.dtype is torch.int64
+        if positions.dim() != 1 or len(positions) != n or not (wide or positions.dtype is torch.int32) or positions.get_device() != self._index:
             raise ValueError(f"positions must be ({n},) int32 or int64 on {self.device}, got {tuple(positions.shape)} "
                              f"{positions.dtype} on {positions.device}")
-        if dim > 1 and x.stride(2) != 1:
+        xs = x.stride()
+        if xs[2] != 1 and dim > 1:
             x = x.contiguous()
+            xs = x.stride()
         if out is None:
-            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            out = torch.empty((n, heads, dim), dtype=x.dtype, device=self.device)
         elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (dim > 1 and out.stride(2) != 1):
             raise ValueError("out must have the shape, type and device of x and contiguous rows")
-        positions = positions.contiguous()
-        xs, ys = x.stride(), out.stride()
-        if self._L.adaptq_rotary_apply(self._ref, x.data_ptr(), xs[0], xs[1], out.data_ptr(), ys[0], ys[1], TYPES[x.dtype],
-                                       positions.data_ptr(), positions.dtype == torch.int64, n, heads, dim, inverse,
-                                       self.device.index, torch.cuda.current_stream(self.device).cuda_stream):
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        ys = out.stride()
+        if self._L.adaptq_rotary_apply(self._ref, x.data_ptr(), xs[0], xs[1], out.data_ptr(), ys[0], ys[1], kind, positions.data_ptr(), wide,
+                                       n, heads, dim, inverse, self._index, current_stream(self._index)):
             raise RuntimeError(_lib.last_error())
         return out
 
 
 class _Rotate(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, positions, rotary):
-        ctx.rotary = rotary
+    def forward(ctx, x, positions, rotary, inverse=0):
+        ctx.rotary, ctx.inverse = rotary, inverse
         ctx.save_for_backward(positions)
-        return rotary._apply(x, positions, None, 0)
+        return rotary._apply(x, positions, None, inverse)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
         positions, = ctx.saved_tensors
-        return ctx.rotary._apply(grad, positions, None, 1), None, None
+        if grad.requires_grad and torch.is_grad_enabled():  # a gradient of the gradient is wanted: rotations all the way
+            return _Rotate.apply(grad, positions, ctx.rotary, 1 - ctx.inverse), None, None, None
+        return ctx.rotary._apply(grad, positions, None, 1 - ctx.inverse), None, None, None
