@@ -8,7 +8,7 @@
 namespace aq {
 
 enum { TYPE_F32 = 0, TYPE_F16 = 1, TYPE_BF16 = 2 };
-enum { PAGED_BAD_PAGE = 1, PAGED_BAD_POSITION = 2, PAGED_GAVE_UP = 4 };
+enum { PAGED_BAD_PAGE = 1, PAGED_BAD_POSITION = 2 };
 
 struct PagedView {
   uint8_t *k_pages, *v_pages;

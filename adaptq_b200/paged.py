@@ -16,8 +16,7 @@ import torch
 from . import _lib
 from .rotary import TYPES, Rotary, current_stream
 
-_STATUS = ((1, "a block table names a page outside the pool"), (2, "a position or length has no room in its block table"),
-           (4, "a kernel gave up waiting for a copy"))
+_STATUS = ((1, "a block table names a page outside the pool"), (2, "a position or length has no room in its block table"))
 
 
 def _padded(dim: int) -> int:

@@ -16,8 +16,8 @@
  *
  * Values that only the device knows are checked there: an entry that would leave the
  * pool or the table is skipped and leaves a bit in *status -- 1: a page number outside the
- * pool, 2: a position or length that the block table has no room for, 4: a kernel gave
- * up waiting for a copy.  The caller zeroes the word and reads it when it likes.
+ * pool, 2: a position or length that the block table has no room for.  The caller zeroes the
+ * word and reads it when it likes.
  */
 #ifndef ADAPTQ_PAGED_H
 #define ADAPTQ_PAGED_H
