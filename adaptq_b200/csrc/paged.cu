@@ -165,12 +165,13 @@ int adaptq_rotary_apply(const adaptq_rotary_t *rotary, const void *x, int64_t x_
           (rotary->interleaved || half % 8 == 0);
   DeviceScope dev(device);
   if (!dev.ok) return fail(fn, "no usable CUDA device (this library has no CPU path)"), -1;
+  // Several tokens a block where there are enough of them: all its threads form turns (16384 tokens x 32 heads x 128,
+  // bf16: 46.4 us with four, 50.1 with one; few tokens would leave SMs idle).
   a.tokens_per_block = 1;
-  a.heads_per_block = n_heads;
+  while (a.tokens_per_block < 4 && a.tokens_per_block * half < ROTARY_THREADS && n_tokens / (2 * a.tokens_per_block) >= 148 * 8) a.tokens_per_block *= 2;
   const long long blocks = (n_tokens + a.tokens_per_block - 1) / a.tokens_per_block;
   if (blocks > 0x7fffffff) return fail(fn, "too many tokens for one call"), -1;
-  rotary_kernel<<<dim3((unsigned)blocks, (n_heads + a.heads_per_block - 1) / a.heads_per_block), ROTARY_THREADS,
-                  a.tokens_per_block * half * sizeof(float2), static_cast<cudaStream_t>(stream)>>>(a);
+  rotary_kernel<<<(unsigned)blocks, ROTARY_THREADS, a.tokens_per_block * half * sizeof(float2), static_cast<cudaStream_t>(stream)>>>(a);
   return launched(fn) ? 0 : -1;
 }
 

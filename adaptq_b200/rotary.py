@@ -106,6 +106,9 @@ class Rotary:
         self._desc = _lib.RotaryDesc(self._turns.data_ptr(), self.factor, self.dim, int(self.interleaved))
         self._ref = C.addressof(self._desc)
 
+    def __reduce__(self):  # copies and pickles make a new one: the descriptor holds device addresses
+        return Rotary, (self.dim, self.base, self.interleaved, self.scaling, str(self.device))
+
     def __call__(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor = None) -> torch.Tensor:
         """x [tokens, heads, dim >= self.dim] (float32, float16 or bfloat16; any strides, the last one 1), positions
         [tokens] (int32 or int64) -> the same shape and type.  `out` may be x (in place).  Differentiable in x (without

@@ -143,6 +143,24 @@ def test_rotary_strides_in_place_and_gradient(gen):
     assert r(torch.empty(0, 5, 64, device="cuda"), pos[:0]).shape == (0, 5, 64)
 
 
+def test_rotary_gradients_of_gradients_and_copies(gen):
+    import copy
+    import pickle
+    from adaptq_b200 import Rotary
+    r = Rotary(24, scaling=SCALINGS[3])
+    x = torch.randn(5, 2, 40, generator=gen, device="cuda", requires_grad=True)
+    pos = torch.arange(3, 8, device="cuda")
+    w = torch.randn(5, 2, 40, generator=gen, device="cuda")
+    (g,) = torch.autograd.grad((r(x, pos) * x.detach()).pow(2).sum(), x, create_graph=True)
+    (h,) = torch.autograd.grad((g * w).sum(), x)   # through both passes: R^T (2 d^2 R w), d = x.detach()
+    d = x.detach().double()
+    want = ref.rotate(2 * d * d * ref.rotate(w.double(), pos, r), pos, r, inverse=True)
+    assert float((h.double() - want).abs().max()) <= 1e-5 * float(want.abs().max())
+    y = r(x.detach(), pos)
+    for other in (copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
+        assert torch.equal(other(x.detach(), pos), y)
+
+
 def test_rotary_refusals(gpu_lib):
     from adaptq_b200 import Rotary
     r = Rotary(64)
@@ -431,7 +449,7 @@ def test_refusals(gpu_lib):
                 lambda: c.append(k, k, table, n.long()), lambda: c.append(k, k, table, n[:1]), lambda: c.append(k, k, table[:1], n[:1]),
                 lambda: c.append(k, k, table, n, n), lambda: c.append(k, k, table, n, rotary=wide), lambda: c.attend(q[:, :3], table, n),
                 lambda: c.attend(q[:1], table, n), lambda: c.attend(q, table, n[:1]), lambda: c.attend(q, table, n, rotary="x"),
-                lambda: c.attend(q, table, n, out=q[:, :2]), lambda: c.attend(q[..., :32], table, n), lambda: c.attend(q.cpu(), table, n),
+                lambda: c.attend(q, table[:, :0], n), lambda: c.append(k, k, table[:, :0], n), lambda: c.attend(q, table, n, out=q[:, :2]), lambda: c.attend(q[..., :32], table, n), lambda: c.attend(q.cpu(), table, n),
                 lambda: c.read(table, n, n, 2), lambda: c.read(table, n, ints(0, 1, 2), 2, dtype=torch.int8),
                 lambda: c.read(table, n, ints(0, 1, 2), 2, out=(k[:1], k[:1]))):
         with pytest.raises(ValueError):
@@ -532,6 +550,34 @@ def test_streams_and_graphs(gen):
     torch.cuda.synchronize()
     assert all(torch.equal(o, alone) for per in got for o in per)
     cache.check()
+
+
+def test_offsets_beyond_32_bits(gen):
+    """A pool of more than 4 GiB a side, pages from its end; rows further than 2^31 elements apart."""
+    from adaptq_b200 import PagedKVCache, Rotary
+    heads, dim = 8, 256
+    signs = ref.random_signs(heads, 256, gen)
+    cache = PagedKVCache(18000, heads, dim, 4, 4, 256, signs=signs)   # 4.7e9 bytes of keys
+    assert cache.k_pages.numel() > 2 ** 32
+    table = ints(17999, 9001, 17000, 5).view(2, 2)
+    k, v = (torch.randn(600, heads, dim, generator=gen, device="cuda") for _ in range(2))
+    rotary = Rotary(dim)
+    cache.append(k, v, table, ints(0, 0), ints(0, 400, 600), rotary=rotary)
+    cache.check()
+    for b, (lo, hi) in enumerate(((0, 400), (400, 600))):
+        check_rows(cache, signs.double(), table[b], 0, k[lo:hi], v[lo:hi], rotary)
+    q = torch.randn(2, heads, dim, generator=gen, device="cuda")
+    attend_close(cache.attend(q, table, ints(400, 200), rotary=rotary), ref.attend(cache, signs.double(), q, table, ints(400, 200), rotary), F32)
+    got, _ = cache.read(table, ints(0, 0), ints(0, 400, 600), 600, dtype=F32)
+    at, off = ref.place(cache, table[0], 400)
+    want, level, norm = ref.rows(cache, "k", at, off, signs.double())
+    close(got[:400], want, 10 * E[F32] * level.abs().sum(-1, keepdim=True) * norm[..., None] / 256 + E[F32] * want.abs())
+    del cache
+    far = torch.zeros(2 ** 31 + 4096, dtype=BF16, device="cuda")
+    x = far.as_strided((2, 2, 64), (2 ** 31, 64, 1))
+    x.copy_(torch.randn(2, 2, 64, generator=gen, device="cuda").to(BF16))
+    r, pos = Rotary(64), torch.tensor([7, 9], device="cuda")
+    assert torch.equal(r(x, pos), r(x.contiguous(), pos))
 
 
 def test_launch_failures_are_errors(gen, gpu_lib):
