@@ -301,9 +301,15 @@ template <int BITS> __device__ __forceinline__ constexpr int code_byte(int i) { 
 
 constexpr int READ_WARPS = 8, READ_TOKENS = 64;
 
+// 16-bit rows that are not made of aligned eights go out through shared memory, eight at a time, so that a warp stores
+// neighbours: [8 rows][4 parts of P/8 words and a gap], which keeps the lanes' words in different banks.
+template <int P> constexpr int stage_part = P / 8 + 1;
+template <int P> constexpr int stage_words = 8 * 4 * stage_part<P>; // of a warp
+
 template <int P, int BITS>
 __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long long dst_token, long long dst_head, int vec,
-                                          const uint8_t *pages, const float *scales, uint32_t (*level)[32], TokenPlace *place) {
+                                          const uint8_t *pages, const float *scales, uint32_t (*level)[32], TokenPlace *place,
+                                          uint32_t *stage) {
   constexpr int N = P / 4, S = N / 2, WORDS = (N * BITS / 8 + 3) / 4;
   const int heads = a.c.heads, dim = a.c.dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const long long t0 = (long long)blockIdx.x * a.block_tokens;
@@ -394,6 +400,25 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
         x[r][s] = __fmul2_rn(x[r][s], make_float2(__uint_as_float(f ^ f0), __uint_as_float(f ^ f1)));
       }
     }
+    if (!vec && a.type != TYPE_F32) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        __syncwarp();
+#pragma unroll
+        for (int s = 0; s < S; ++s) stage[(g * 4 + t) * stage_part<P> + s] = pack2(x[r][s].x, x[r][s].y, a.type);
+        __syncwarp();
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          const int row = 16 * tile + 8 * r + i;
+          if (row >= nt || place[row].page < 0) continue;
+          uint16_t *to = static_cast<uint16_t *>(dst) + (t0 + row) * dst_token + h * dst_head;
+          const uint16_t *from = reinterpret_cast<const uint16_t *>(stage + i * 4 * stage_part<P>);
+#pragma unroll 1
+          for (int d = lane; d < dim; d += 32) to[d] = from[d + 2 * (d / N)];
+        }
+      }
+      continue;
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = 16 * tile + g + 8 * r;
@@ -421,7 +446,7 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
       }); else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          if (t * N + i < dim) store_one(dst, at + i, a.type, (i & 1) ? x[r][i >> 1].y : x[r][i >> 1].x);
+          if (t * N + i < dim) static_cast<float *>(dst)[at + i] = (i & 1) ? x[r][i >> 1].y : x[r][i >> 1].x;
       }
     }
   }
@@ -431,10 +456,12 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
 template <int P, int KB, int VB> __global__ void __launch_bounds__(READ_WARPS * 32) paged_read_kernel(const RowsLaunch a) {
   __shared__ uint32_t level[16][32];
   __shared__ TokenPlace place[READ_TOKENS];
+  __shared__ uint32_t stage[READ_WARPS * stage_words<P>];
+  uint32_t *mine = stage + (threadIdx.x >> 5) * stage_words<P>;
   if (blockIdx.y == 0)
-    read_rows<P, KB>(a, a.k, a.k_token, a.k_head, a.k_vec, a.c.k_pages, a.c.k_scales, level, place);
+    read_rows<P, KB>(a, a.k, a.k_token, a.k_head, a.k_vec, a.c.k_pages, a.c.k_scales, level, place, mine);
   else
-    read_rows<P, VB>(a, a.v, a.v_token, a.v_head, a.v_vec, a.c.v_pages, a.c.v_scales, level, place);
+    read_rows<P, VB>(a, a.v, a.v_token, a.v_head, a.v_vec, a.c.v_pages, a.c.v_scales, level, place, mine);
 }
 
 } // namespace aq
