@@ -4,7 +4,7 @@
 // (sequence, KV head, pass of up to eight of its queries).  All units of the call, in that
 // order, are cut into equal runs, one per warp of a persistent grid, wherever the cuts fall;
 // the lengths are read on the device.  A warp works alone: it fetches its units into a ring of
-// two (16-byte asynchronous copies), keeps its own running maximum and sum, and meets no barrier
+// two (16-byte asynchronous copies), keeps its own reference and sums, and meets no barrier
 // with other warps until it is done.  A run that starts or ends inside an item leaves a partial
 // result; a block joins those of its warps when all are done, and paged_join_kernel those of
 // items that span blocks.  (Joining those too in this kernel, by the last block to arrive, saves
@@ -53,7 +53,6 @@ template <int KB, int VB, int P, int MODE> struct AttendShape {
   static constexpr int K_ROW = P * KB / 8, V_ROW = P * VB / 8;
   static constexpr int STAGE = U * (K_ROW + V_ROW + 8);
   static constexpr int COLS = SPLIT ? 4 : 8; // queries of a pass
-  static constexpr int ROUNDS = EXACT ? 1 : U / 32; // unrolled: EXACT would not fit the instruction cache
   static constexpr int table_bytes(int bits) { return bits == 2 && !EXACT ? 32768 : 128 << (2 * bits); }
   static constexpr int K_TABLE = 0, V_TABLE = KB == VB ? 0 : table_bytes(KB);
   static constexpr int TABLES = table_bytes(KB) + (KB == VB ? 0 : table_bytes(VB));
@@ -70,7 +69,6 @@ template <int KB, int VB, int P, int MODE> struct AttendShape {
   static constexpr int SMEM = BLOCK + FIXED;
   static_assert(WARPS >= 4 && SMEM <= ATTEND_SMEM, "shared memory");
   static_assert(STAGE >= 16 * P, "finish() puts four columns there");
-  static_assert(WARPS >= 3 && SMEM <= ATTEND_SMEM, "shared memory");
 };
 
 // Length of sequence b as far as its table has room.
@@ -85,7 +83,7 @@ __device__ __forceinline__ int clipped_length(const AttendLaunch &a, int b, bool
 __device__ __forceinline__ int slot_floats(int cols, int P) { return cols * (P + 4); }
 
 // The factor by which the tables' values are larger than the codebook's: of all factors from 1 to 2, the one
-// whose largest rounding error to float16 is smallest (1.7e-8, 3.7e-6 and 1.0e-4 of a value; without it 2.6e-4 to
+// whose largest rounding error to float16 is smallest (1.7e-8, 3.7e-6 and 1.0e-4 of a value; without it 2.3e-4 to
 // 4.3e-4).
 __host__ __device__ constexpr float table_scale(int bits) { return bits == 2 ? 1.2207031f : bits == 3 ? 1.1793699f : 1.57108554f; }
 
@@ -213,72 +211,74 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
     const uint8_t *keys = attend_smem + stage, *vals = keys + U * S::K_ROW;
     const float *ks = reinterpret_cast<const float *>(attend_smem + stage + U * (S::K_ROW + S::V_ROW)), *vs = ks + U;
     float s[TILES][4];
+    // two tiles a round; with the codebook in two parts unrolled rounds would not stay in the instruction cache (rolled, and
+    // with tables half the size, 20 x 6 heads of 96 coordinates went from 49 to 37 us)
 #pragma unroll (EXACT ? 1 : TILES / 2)
     for (int round = 0; round < TILES / 2; ++round) {
 #pragma unroll
-    for (int i = 0; i + 2 < TILES; ++i) {
+      for (int i = 0; i + 2 < TILES; ++i) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = s[i + 2][j];
-    }
-#pragma unroll
-    for (int i = TILES - 2; i < TILES; ++i) {
-      const uint8_t *tile = keys + (32 * round + 16 * (i - TILES + 2) + phi) * S::K_ROW + t * K_PART;
-      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-      uint32_t w[2][K_WORDS], g24[2][KB == 3 ? P / 32 : 1];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        load_packed<K_PART>(tile + 8 * r * S::K_ROW, w[r]);
-        if constexpr (KB == 3) {
-#pragma unroll
-          for (int k = 0; k < P / 32; ++k) g24[r][k] = spread6(group24<K_WORDS>(w[r], k));
-        }
+        for (int j = 0; j < 4; ++j) s[i][j] = s[i + 2][j];
       }
-      if constexpr (KB == 2 && !EXACT) {
-        // a byte: two codes of one row and two of the other, an entry: the operands of both
 #pragma unroll
-        for (int k = 0; k < K_WORDS; ++k) {
-          const uint32_t x = (w[0][k] & 0xf0f0f0f0u) | ((w[1][k] >> 4) & 0x0f0f0f0fu), y = ((w[0][k] << 4) & 0xf0f0f0f0u) | (w[1][k] & 0x0f0f0f0fu);
+      for (int i = TILES - 2; i < TILES; ++i) {
+        const uint8_t *tile = keys + (32 * round + 16 * (i - TILES + 2) + phi) * S::K_ROW + t * K_PART;
+        s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        uint32_t w[2][K_WORDS], g24[2][KB == 3 ? P / 32 : 1];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint2 u = table_two(entry_address<8, 7>(k_table, x, 8 * j)), v = table_two(entry_address<8, 7>(k_table, y, 8 * j));
-            mma_16816(s[i], u.x, u.y, v.x, v.y, qb[8 * k + 2 * j], qb[8 * k + 2 * j + 1]);
+        for (int r = 0; r < 2; ++r) {
+          load_packed<K_PART>(tile + 8 * r * S::K_ROW, w[r]);
+          if constexpr (KB == 3) {
+#pragma unroll
+            for (int k = 0; k < P / 32; ++k) g24[r][k] = spread6(group24<K_WORDS>(w[r], k));
           }
         }
-      } else {
-        float odd[4] = {}, low[4] = {}; // EXACT
+        if constexpr (KB == 2 && !EXACT) {
+          // a byte: two codes of one row and two of the other, an entry: the operands of both
 #pragma unroll
-        for (int k = 0; k < DIM_TILES; ++k) {
-          uint32_t word[2][2];
-          int pos[2];
+          for (int k = 0; k < K_WORDS; ++k) {
+            const uint32_t x = (w[0][k] & 0xf0f0f0f0u) | ((w[1][k] >> 4) & 0x0f0f0f0fu), y = ((w[0][k] << 4) & 0xf0f0f0f0u) | (w[1][k] & 0x0f0f0f0fu);
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+            for (int j = 0; j < 4; ++j) {
+              const uint2 u = table_two(entry_address<8, 7>(k_table, x, 8 * j)), v = table_two(entry_address<8, 7>(k_table, y, 8 * j));
+              mma_16816(s[i], u.x, u.y, v.x, v.y, qb[8 * k + 2 * j], qb[8 * k + 2 * j + 1]);
+            }
+          }
+        } else {
+          float odd[4] = {}, low[4] = {}; // EXACT
 #pragma unroll
-            for (int p = 0; p < 2; ++p) word[r][p] = key_word(w[r], g24[r], 2 * k + p, pos[p]);
+          for (int k = 0; k < DIM_TILES; ++k) {
+            uint32_t word[2][2];
+            int pos[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int p = 0; p < 2; ++p) word[r][p] = key_word(w[r], g24[r], 2 * k + p, pos[p]);
+            if constexpr (EXACT) {
+              uint2 v[2][2];
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) v[r][p] = table_two(entry_address<2 * KB, 7>(k_table, word[r][p], pos[p]));
+              // The tensor cores cut sums off instead of rounding them: short chains, added up in float32.
+              if (k & 1) mma_16816(odd, v[0][0].x, v[1][0].x, v[0][1].x, v[1][1].x, qb[2 * k], qb[2 * k + 1]);
+              else mma_16816(s[i], v[0][0].x, v[1][0].x, v[0][1].x, v[1][1].x, qb[2 * k], qb[2 * k + 1]);
+              mma_16816(low, v[0][0].y, v[1][0].y, v[0][1].y, v[1][1].y, qb[2 * k], qb[2 * k + 1]);
+            } else {
+              uint32_t v[2][2];
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) v[r][p] = table_one(entry_address<2 * KB, 7>(k_table, word[r][p], pos[p]));
+              mma_16816(s[i], v[0][0], v[1][0], v[0][1], v[1][1], qb[2 * k], qb[2 * k + 1]);
+            }
+          }
           if constexpr (EXACT) {
-            uint2 v[2][2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int p = 0; p < 2; ++p) v[r][p] = table_two(entry_address<2 * KB, 7>(k_table, word[r][p], pos[p]));
-            // The tensor cores cut sums off instead of rounding them: short chains, added up in float32.
-            if (k & 1) mma_16816(odd, v[0][0].x, v[1][0].x, v[0][1].x, v[1][1].x, qb[2 * k], qb[2 * k + 1]);
-            else mma_16816(s[i], v[0][0].x, v[1][0].x, v[0][1].x, v[1][1].x, qb[2 * k], qb[2 * k + 1]);
-            mma_16816(low, v[0][0].y, v[1][0].y, v[0][1].y, v[1][1].y, qb[2 * k], qb[2 * k + 1]);
-          } else {
-            uint32_t v[2][2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int p = 0; p < 2; ++p) v[r][p] = table_one(entry_address<2 * KB, 7>(k_table, word[r][p], pos[p]));
-            mma_16816(s[i], v[0][0], v[1][0], v[0][1], v[1][1], qb[2 * k], qb[2 * k + 1]);
+            for (int j = 0; j < 4; ++j) s[i][j] += odd[j] + low[j];
           }
         }
-        if constexpr (EXACT) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][j] += odd[j] + low[j];
-        }
       }
-    }
     }
     // softmax: s becomes the logit over fq, then weight times the value's norm
     float top[2] = {-1e30f, -1e30f}, norm[TILES][2], largest = 0.f; // largest: norm of this lane's values
@@ -345,77 +345,77 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
 #pragma unroll (EXACT ? 1 : TILES / 2)
     for (int round = 0; round < TILES / 2; ++round) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint8_t *tile = vals + (32 * round + 16 * i) * S::V_ROW + g * V_PART;
-      uint32_t wt[2];
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t *tile = vals + (32 * round + 16 * i) * S::V_ROW + g * V_PART;
+        uint32_t wt[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float x = s[i][2 * r], y = s[i][2 * r + 1];
-        uint32_t w = half2_bits(x, y);
-        if constexpr (SPLIT) {
-          const float2 upper = unpack2(w, TYPE_F16);
-          const uint32_t lower = half2_bits(x - upper.x, y - upper.y);
-          w = t >= 2 ? lower : w;
+        for (int r = 0; r < 2; ++r) {
+          const float x = s[i][2 * r], y = s[i][2 * r + 1];
+          uint32_t w = half2_bits(x, y);
+          if constexpr (SPLIT) {
+            const float2 upper = unpack2(w, TYPE_F16);
+            const uint32_t lower = half2_bits(x - upper.x, y - upper.y);
+            w = t >= 2 ? lower : w;
+          }
+          wt[r] = transpose_8x8(w);
         }
-        wt[r] = transpose_8x8(w);
-      }
-      // the codes of one coordinate of two tokens side by side: even coordinates in x, odd ones in y
-      uint32_t x[2][VB == 3 ? P / 64 : V_WORDS], y[2][VB == 3 ? P / 64 : V_WORDS];
+        // the codes of one coordinate of two tokens side by side: even coordinates in x, odd ones in y
+        uint32_t x[2][VB == 3 ? P / 64 : V_WORDS], y[2][VB == 3 ? P / 64 : V_WORDS];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        uint32_t wa[V_WORDS], wb[V_WORDS];
-        load_packed<V_PART>(tile + (8 * r + t) * S::V_ROW, wa);
-        load_packed<V_PART>(tile + (8 * r + 7 - t) * S::V_ROW, wb);
-        if constexpr (VB == 3) {
+        for (int r = 0; r < 2; ++r) {
+          uint32_t wa[V_WORDS], wb[V_WORDS];
+          load_packed<V_PART>(tile + (8 * r + t) * S::V_ROW, wa);
+          load_packed<V_PART>(tile + (8 * r + 7 - t) * S::V_ROW, wb);
+          if constexpr (VB == 3) {
 #pragma unroll
-          for (int k = 0; k < P / 64; ++k) {
-            const uint32_t va = group24<V_WORDS>(wa, k), vb = group24<V_WORDS>(wb, k);
-            x[r][k] = spread6((va & 070707070) | ((vb >> 3) & 007070707));
-            y[r][k] = spread6(((va << 3) & 070707070) | (vb & 007070707));
+            for (int k = 0; k < P / 64; ++k) {
+              const uint32_t va = group24<V_WORDS>(wa, k), vb = group24<V_WORDS>(wb, k);
+              x[r][k] = spread6((va & 070707070) | ((vb >> 3) & 007070707));
+              y[r][k] = spread6(((va << 3) & 070707070) | (vb & 007070707));
+            }
+          } else {
+            constexpr uint32_t HI = VB == 4 ? 0xf0f0f0f0u : 0xccccccccu;
+#pragma unroll
+            for (int k = 0; k < V_WORDS; ++k) {
+              x[r][k] = (wa[k] & HI) | ((wb[k] >> VB) & ~HI);
+              y[r][k] = ((wa[k] << VB) & HI) | (wb[k] & ~HI);
+            }
+          }
+        }
+        if constexpr (VB == 2 && !EXACT) {
+#pragma unroll
+          for (int j = 0; j < DIM_TILES; j += 2) { // a byte: coordinates 2j and 2j+2, or 2j+1 and 2j+3 (rows g and g+8)
+            const uint2 a = table_two(entry_address<8, 7>(v_table, x[0][j >> 3], 8 * ((j >> 1) & 3))), b = table_two(entry_address<8, 7>(v_table, x[1][j >> 3], 8 * ((j >> 1) & 3)));
+            mma_16816(acc[j], a.x, a.y, b.x, b.y, wt[0], wt[1]);
+            const uint2 c = table_two(entry_address<8, 7>(v_table, y[0][j >> 3], 8 * ((j >> 1) & 3))), d = table_two(entry_address<8, 7>(v_table, y[1][j >> 3], 8 * ((j >> 1) & 3)));
+            mma_16816(acc[j + 1], c.x, c.y, d.x, d.y, wt[0], wt[1]);
           }
         } else {
-          constexpr uint32_t HI = VB == 4 ? 0xf0f0f0f0u : 0xccccccccu;
 #pragma unroll
-          for (int k = 0; k < V_WORDS; ++k) {
-            x[r][k] = (wa[k] & HI) | ((wb[k] >> VB) & ~HI);
-            y[r][k] = ((wa[k] << VB) & HI) | (wb[k] & ~HI);
+          for (int j = 0; j < DIM_TILES; ++j) {
+            const int k = VB == 4 || VB == 3 ? j >> 2 : j >> 3;
+            const int pos = VB == 4 ? 8 * (j & 3) : VB == 3 ? 24 - 8 * (j & 3) : 8 * ((j >> 1) & 3) + ((j & 1) ? 0 : 4);
+            const uint32_t src[4] = {x[0][k], y[0][k], x[1][k], y[1][k]};
+            if constexpr (EXACT) {
+              uint2 v[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) v[q] = table_two(entry_address<2 * VB, 7>(v_table, src[q], pos));
+              mma_16816(acc[j], v[0].x, v[1].x, v[2].x, v[3].x, wt[0], wt[1]);
+              mma_16816(acc[j], v[0].y, v[1].y, v[2].y, v[3].y, wt[0], wt[1]);
+            } else {
+              uint32_t v[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) v[q] = table_one(entry_address<2 * VB, 7>(v_table, src[q], pos));
+              mma_16816(acc[j], v[0], v[1], v[2], v[3], wt[0], wt[1]);
+            }
           }
         }
       }
-      if constexpr (VB == 2 && !EXACT) {
 #pragma unroll
-        for (int j = 0; j < DIM_TILES; j += 2) { // a byte: coordinates 2j and 2j+2, or 2j+1 and 2j+3 (rows g and g+8)
-          const uint2 a = table_two(entry_address<8, 7>(v_table, x[0][j >> 3], 8 * ((j >> 1) & 3))), b = table_two(entry_address<8, 7>(v_table, x[1][j >> 3], 8 * ((j >> 1) & 3)));
-          mma_16816(acc[j], a.x, a.y, b.x, b.y, wt[0], wt[1]);
-          const uint2 c = table_two(entry_address<8, 7>(v_table, y[0][j >> 3], 8 * ((j >> 1) & 3))), d = table_two(entry_address<8, 7>(v_table, y[1][j >> 3], 8 * ((j >> 1) & 3)));
-          mma_16816(acc[j + 1], c.x, c.y, d.x, d.y, wt[0], wt[1]);
-        }
-      } else {
+      for (int i = 0; i + 2 < TILES; ++i) {
 #pragma unroll
-        for (int j = 0; j < DIM_TILES; ++j) {
-          const int k = VB == 4 || VB == 3 ? j >> 2 : j >> 3;
-          const int pos = VB == 4 ? 8 * (j & 3) : VB == 3 ? 24 - 8 * (j & 3) : 8 * ((j >> 1) & 3) + ((j & 1) ? 0 : 4);
-          const uint32_t src[4] = {x[0][k], y[0][k], x[1][k], y[1][k]};
-          if constexpr (EXACT) {
-            uint2 v[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = table_two(entry_address<2 * VB, 7>(v_table, src[q], pos));
-            mma_16816(acc[j], v[0].x, v[1].x, v[2].x, v[3].x, wt[0], wt[1]);
-            mma_16816(acc[j], v[0].y, v[1].y, v[2].y, v[3].y, wt[0], wt[1]);
-          } else {
-            uint32_t v[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = table_one(entry_address<2 * VB, 7>(v_table, src[q], pos));
-            mma_16816(acc[j], v[0], v[1], v[2], v[3], wt[0], wt[1]);
-          }
-        }
+        for (int j = 0; j < 4; ++j) s[i][j] = s[i + 2][j];
       }
-    }
-#pragma unroll
-    for (int i = 0; i + 2 < TILES; ++i) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = s[i + 2][j];
-    }
     }
   }
 
