@@ -308,9 +308,10 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
 #pragma unroll
       for (int e = 0; e < 2; ++e) top[e] = fmaxf(top[e], fmaxf(s[i][e], s[i][2 + e]));
     }
-    // The reference stays as long as no weight exceeds 2^100 and no weight times norm 2^10 (it is at most 1 where the
-    // reference was set: float16 then holds all that counts beside it).
-    const float room = fminf(100.f, 10.f - __log2f(largest));
+    // The reference stays as long as no weight exceeds 2^100 and no weight times norm 2^15.  Where it is set, the largest
+    // weight times norm becomes 2^9: float16 then holds everything down to 2^-33 of that one, so that very many tokens
+    // far below a single one still add up.
+    const float room = fminf(100.f, 15.f - __log2f(largest));
     if (__any_sync(0xffffffffu, fmaf(top[0], fq[0], -ref[0]) > room || fmaf(top[1], fq[1], -ref[1]) > room)) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -324,7 +325,7 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
           for (int r = 0; r < 2; ++r) product = fmaxf(product, fmaf(s[i][2 * r + e], fq[e], -high) + __log2f(norm[i][r]));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) product = fmaxf(product, __shfl_xor_sync(0xffffffffu, product, o));
-        const float next = fmaxf(ref[e], high + product), ratio = exp2_approx(ref[e] - next);
+        const float next = fmaxf(ref[e], high + product - 9.f), ratio = exp2_approx(ref[e] - next);
         ref[e] = next;
         l[e] *= ratio;
 #pragma unroll

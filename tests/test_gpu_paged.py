@@ -435,6 +435,39 @@ def test_attend_extremes(gen, dtype):
     assert bool(bad[1].isnan().all()) and torch.equal(bad[[0, 2, 3]], got[[0, 2, 3]])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("power", [10, 20, 27])
+def test_many_tokens_far_below_one(gen, dtype, power):
+    """One value 2^power times as long as 30000 equal ones under equal weights: their sum still counts."""
+    cache, signs = make_cache(gen, 118, 1, 128, 4, 4, 256)
+    ref.random_pool(cache, gen)
+    cache.k_scales.zero_()                                   # equal logits
+    cache.v_pages[:] = cache.v_pages[0, 0, 0]                # one row for all
+    cache.v_scales.fill_(1.0)
+    table = ref.random_table(cache, [30000], gen)
+    page = int(table[0, 7])
+    cache.v_scales[page, 0, 11] = 2.0 ** power
+    cache.v_pages[page, 0, 11] = cache.v_pages[page, 0, 11].flip(0)   # another direction
+    q = torch.randn(1, 1, 128, generator=gen, device="cuda").to(dtype)
+    got, want = cache.attend(q, table, ints(30000)), ref.attend(cache, signs, q, table, ints(30000))
+    attend_close(got, want, dtype)
+
+
+def test_shared_pages_and_views(gen):
+    """Sequences that share their first pages; tables, lengths and queries that are views; the output in the queries' place."""
+    cache, signs = make_cache(gen, 20, 2, 64, 4, 2, 16)
+    ref.random_pool(cache, gen)
+    wide = torch.full((6, 9), -1, dtype=torch.int32, device="cuda")
+    wide[::2, 2:8] = torch.tensor([[3, 4, 5, 6, 7, 8], [3, 4, 9, 10, 11, 12], [3, 4, 5, 6, 13, 13]], dtype=torch.int32, device="cuda")
+    table, n = wide[::2, 2:], ints(90, 0, 40, 0, 96, 0)[::2]
+    q = torch.randn(3, 2, 5, 64, generator=gen, device="cuda").to(BF16).transpose(1, 2).reshape(3, 10, 64)
+    want = ref.attend(cache, signs, q, table, n)
+    attend_close(cache.attend(q, table, n), want, BF16)
+    assert torch.equal(cache.attend(q, table, n, out=q), q)
+    attend_close(q, want, BF16)
+    cache.check()
+
+
 def test_refusals(gpu_lib):
     from adaptq_b200 import PagedKVCache, Rotary
     for bad in (dict(dim=32), dict(dim=257), dict(k_bits=5), dict(v_bits=16), dict(page_size=48), dict(n_pages=0), dict(n_kv_heads=0), dict(device="cpu"),
