@@ -30,6 +30,8 @@ struct DeviceScope { // the call's device is current while this lives
 bool fail(const char *fn, const char *what) { aq_set_error("%s: %s", fn, what); return false; }
 
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+// Addresses that the kernels could not read or write element by element.
+template <typename... T> bool misaligned(size_t n, const T *...p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & (n - 1)) != 0; }
 int size_of(int type) { return type == TYPE_F32 ? 4 : 2; }
 int padded_of(int dim) { int p = 64; while (p < dim) p <<= 1; return p; }
 
@@ -49,6 +51,7 @@ bool check_cache(const char *fn, const adaptq_paged_t *c, PagedView &v) {
   if (c->n_pages <= 0 || c->n_pages > 0x7fffffff || c->n_kv_heads <= 0 || c->n_kv_heads > 65535) return fail(fn, "invalid number of pages or heads");
   if (!aligned(c->k_pages, 16) || !aligned(c->v_pages, 16) || !aligned(c->k_scales, 16) || !aligned(c->v_scales, 16))
     return fail(fn, "pages and scales must be 16-byte aligned");
+  if (misaligned(4, c->signs, c->status)) return fail(fn, "a pointer in the cache is not aligned to its elements");
   int shift = 4;
   while ((1 << shift) < c->page_size) ++shift;
   v = PagedView{static_cast<uint8_t *>(c->k_pages), static_cast<uint8_t *>(c->v_pages), c->k_scales, c->v_scales, c->signs, c->status,
@@ -59,7 +62,7 @@ bool check_cache(const char *fn, const adaptq_paged_t *c, PagedView &v) {
 bool check_rotary(const char *fn, const adaptq_rotary_t *r, int dim, RotaryView &v) {
   v = RotaryView{nullptr, 1.f, 0, 0};
   if (!r) return true;
-  if (!r->turns) return fail(fn, "null rotary frequencies");
+  if (!r->turns || misaligned(8, r->turns)) return fail(fn, "null or unaligned rotary frequencies");
   if (r->dim < 2 || r->dim % 2 || r->dim > dim) return fail(fn, "the rotary dimension must be even and at most the head dimension");
   v = RotaryView{reinterpret_cast<const unsigned long long *>(r->turns), r->factor, r->dim, r->interleaved != 0};
   return true;
@@ -110,6 +113,7 @@ int rows_call(const char *fn, bool append, const adaptq_paged_t *cache, void *k,
   if (n_seqs < 0 || n_tokens < 0 || table_width < 0) return fail(fn, "negative size"), -1;
   if (n_seqs == 0 || n_tokens == 0) return 0;
   if (!k || !v || !table || !starts) return fail(fn, "null pointer"), -1;
+  if (misaligned(size_of(type), k, v) || misaligned(4, table, starts, cu_tokens)) return fail(fn, "a pointer is not aligned to its elements"), -1;
   const int P = padded_of(cache->dim);
   if (n_tokens > (1ll << 31) / cache->n_kv_heads) return fail(fn, "too many tokens for one call"), -1;
   a.table = TableView{table, table_stride, table_width};
@@ -156,6 +160,7 @@ int adaptq_rotary_apply(const adaptq_rotary_t *rotary, const void *x, int64_t x_
   if (!check_rotary(fn, rotary, dim, a.r) || !check_type(fn, type)) return -1;
   if (n_tokens == 0 || n_heads == 0) return 0;
   if (!x || !y || !positions) return fail(fn, "null pointer"), -1;
+  if (misaligned(size_of(type), x, y) || misaligned(positions_64 ? 8 : 4, positions)) return fail(fn, "a pointer is not aligned to its elements"), -1;
   const int half = rotary->dim / 2;
   if (half * (int)sizeof(float2) > 32768) return fail(fn, "rotary dimensions above 8192 are not supported"), -1;
   a.x = x; a.y = y; a.positions = positions; a.positions_64 = positions_64 != 0;
@@ -226,6 +231,7 @@ int adaptq_paged_attend(const adaptq_paged_t *cache, const void *q, int64_t q_se
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(fn, "scale must be positive and finite"), -1;
   if (n_seqs == 0) return 0;
   if (!q || !out || !table || !lengths) return fail(fn, "null pointer"), -1;
+  if (misaligned(size_of(type), q, out) || misaligned(4, table, lengths)) return fail(fn, "a pointer is not aligned to its elements"), -1;
   if (n_q_heads > 1 << 20) return fail(fn, "at most 1048576 query heads are supported"), -1;
   if (n_q_heads / cache->n_kv_heads > 65536) return fail(fn, "at most 65536 queries per KV head are supported"), -1;
   if ((long long)n_seqs * n_q_heads > 0x3fffffff) return fail(fn, "too many sequences for one call"), -1;

@@ -11,8 +11,8 @@
  *
  * All pointers are DEVICE memory of the device `adaptq_paged_t.device` unless stated.
  * Element types: 0 = float32, 1 = float16, 2 = bfloat16.  Strides count elements; the
- * last dimension of every tensor is contiguous.  `stream` is a cudaStream_t (NULL = the
- * default stream).  Functions return 0, or -1 and set adaptq_last_error().
+ * last dimension of every tensor is contiguous, pointers are aligned to their elements.
+ * `stream` is a cudaStream_t (NULL = the default stream).  Functions return 0, or -1 and set adaptq_last_error().
  *
  * Values that only the device knows are checked there: an entry that would leave the
  * pool or the table is skipped and leaves a bit in *status -- 1: a page number outside the
@@ -87,8 +87,10 @@ int adaptq_paged_read(const adaptq_paged_t *cache, void *k_out, int64_t k_token_
  * [n_seqs][n_q_heads][dim], query head j reading KV head j / (n_q_heads / n_kv_heads).
  * Logits are scale * q.k (scale > 0; the rings' is 1 / sqrt(dim)); queries are rotated by
  * position lengths[b] - 1 first, if `rotary`.  A sequence of length 0 gives zeros.  float32
- * calls are computed in float32 throughout; the 16-bit types multiply in float16 with
- * float32 sums.
+ * calls are computed to float32's precision throughout (codebook, queries and weights in two
+ * float16 parts); float16 calls hold queries and weights in two parts, bfloat16 calls in one;
+ * sums are float32.  Tokens are taken 64 at a time (32 above 128 coordinates): one page that
+ * does not exist leaves all of its 64 out.
  * workspace: adaptq_paged_attend_workspace() bytes, 16-byte aligned, whose contents need not
  * be kept between calls; calls that may overlap need one each. */
 size_t adaptq_paged_attend_workspace(const adaptq_paged_t *cache, int n_seqs, int n_q_heads, int type);

@@ -70,10 +70,15 @@ def test_bad_calls(lib):
     assert attend(lib, d, q=None) == -1 and "null pointer" in err()
     assert attend(lib, d, size=0) == -1 and "workspace" in err()
     assert attend(lib, d, n_seqs=0) == 0
+    assert append(lib, d, k=4097) == -1 and "aligned" in err()
+    assert append(lib, d, k=4098, type=0) == -1 and "aligned" in err()
+    assert attend(lib, d, q=4097, type=2) == -1 and "aligned" in err()
+    assert append(lib, desc(status=4098)) == -1 and "aligned" in err()
+    assert append(lib, d, rot=rotary(turns=4100)) == -1 and "rotary" in err()
     r = rotary()
     args = lambda **k: [C.addressof(k.get("r", r)), k.get("x", 4096), 64, 64, 4096, 64, 64, k.get("type", 0), 4096, 0, k.get("n", 1), k.get("h", 1),  # noqa: E731
                         k.get("dim", 64), 0, 0, None]
-    for bad in (dict(x=None), dict(type=7), dict(n=-1), dict(h=-1), dict(dim=0), dict(dim=62), dict(r=rotary(dim=3))):
+    for bad in (dict(x=None), dict(x=4097), dict(x=4098), dict(type=7), dict(n=-1), dict(h=-1), dict(dim=0), dict(dim=62), dict(r=rotary(dim=3))):
         assert lib.adaptq_rotary_apply(*args(**bad)) == -1 and err()
     assert lib.adaptq_rotary_apply(*args(n=0)) == 0
 
