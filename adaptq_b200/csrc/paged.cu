@@ -176,7 +176,9 @@ int adaptq_rotary_apply(const adaptq_rotary_t *rotary, const void *x, int64_t x_
   while (a.tokens_per_block < 4 && a.tokens_per_block * half < ROTARY_THREADS && n_tokens / (2 * a.tokens_per_block) >= 148 * 8) a.tokens_per_block *= 2;
   const long long blocks = (n_tokens + a.tokens_per_block - 1) / a.tokens_per_block;
   if (blocks > 0x7fffffff) return fail(fn, "too many tokens for one call"), -1;
-  rotary_kernel<<<(unsigned)blocks, ROTARY_THREADS, a.tokens_per_block * half * sizeof(float2), static_cast<cudaStream_t>(stream)>>>(a);
+  a.heads_per_block = std::min(n_heads, (1 << 28) / dim); // all heads, as long as they are below 2^28 coordinates
+  const unsigned head_blocks = (unsigned)((n_heads + a.heads_per_block - 1) / a.heads_per_block);
+  rotary_kernel<<<dim3((unsigned)blocks, head_blocks), ROTARY_THREADS, a.tokens_per_block * half * sizeof(float2), static_cast<cudaStream_t>(stream)>>>(a);
   return launched(fn) ? 0 : -1;
 }
 

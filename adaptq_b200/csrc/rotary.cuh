@@ -15,7 +15,7 @@ struct RotaryLaunch {
   const void *positions;
   long long x_token, x_head, y_token, y_head, n_tokens;
   int heads, dim, type, positions_64, inverse;
-  int tokens_per_block;
+  int tokens_per_block, heads_per_block; // whose product with dim stays within 2^30: a block counts in 32 bits
   int vec; // rows are 16-byte aligned and whole eights, and so are the halves
 };
 
@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
   const int half = a.r.dim >> 1;
   const long long t0 = (long long)blockIdx.x * a.tokens_per_block;
   const int nt = (int)min((long long)a.tokens_per_block, a.n_tokens - t0);
+  const int h0 = blockIdx.y * a.heads_per_block, heads = min(a.heads_per_block, a.heads - h0);
   for (int i = threadIdx.x; i < nt * half; i += ROTARY_THREADS) {
     const int t = i / half, pair = i - t * half;
     const long long pos = a.positions_64 ? static_cast<const long long *>(a.positions)[t0 + t]
@@ -39,9 +40,9 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
     constexpr int TYPE = decltype(type)::value;
     // one thread: eight neighbours and, in the half layout, their eight partners
     const int parts = a.r.interleaved ? a.dim >> 3 : (a.dim - half) >> 3;
-    const int n = nt * a.heads * parts;
+    const int n = nt * heads * parts;
     for (int i = threadIdx.x; i < n; i += ROTARY_THREADS) {
-      const int part = i % parts, th = i / parts, h = th % a.heads, t = th / a.heads;
+      const int part = i % parts, th = i / parts, h = h0 + th % heads, t = th / heads;
       const long long xi = (t0 + t) * a.x_token + h * a.x_head, yi = (t0 + t) * a.y_token + h * a.y_head;
       const float2 *cs = rotary_turns + t * half;
       float u[8], w[8];
@@ -77,9 +78,9 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
     }
   }); else {
     // one thread: one pair, or one element behind the rotated part
-    const int parts = a.dim - half, n = nt * a.heads * parts;
+    const int parts = a.dim - half, n = nt * heads * parts;
     for (int i = threadIdx.x; i < n; i += ROTARY_THREADS) {
-      const int part = i % parts, th = i / parts, h = th % a.heads, t = th / a.heads;
+      const int part = i % parts, th = i / parts, h = h0 + th % heads, t = th / heads;
       const long long xi = (t0 + t) * a.x_token + h * a.x_head, yi = (t0 + t) * a.y_token + h * a.y_head;
       if (part < half) {
         const int d = a.r.interleaved ? 2 * part : part, e = a.r.interleaved ? d + 1 : d + half;
