@@ -109,6 +109,7 @@ SYMBOLS = {
     "adaptq_rotary_apply": (C.c_int, [C.c_void_p, *_rows, *_rows, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int,
                                       C.c_int, C.c_void_p]),
     "adaptq_paged_signs": (C.c_int, [C.c_uint64, C.c_int, C.c_int, C.c_void_p]),
+    "adaptq_paged_take_status": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "adaptq_paged_append": (C.c_int, [C.c_void_p, *_rows, *_rows, C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int,
                                       C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p]),
     "adaptq_paged_read": (C.c_int, [C.c_void_p, *_rows, *_rows, C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p,

@@ -145,6 +145,9 @@ const attend_unit_t attend_units[3][3] = {{aq_attend_2_2, aq_attend_2_3, aq_atte
 // us instead of 33.6 for 33 x 14 heads of one query; above four queries the further passes cost their share).  bfloat16: one part, eight queries a pass; its output rounding is eight times coarser.
 int attend_mode(int type) { return type == TYPE_F32 ? ATTEND_EXACT : type == TYPE_F16 ? ATTEND_SPLIT : ATTEND_EIGHT; }
 
+// One exchange, so that a bit set by a call on another stream is either taken or left for the next time.
+__global__ void take_status_kernel(int *status, int *taken) { *taken = atomicExch(status, 0); }
+
 } // namespace
 
 extern "C" {
@@ -190,6 +193,19 @@ int adaptq_paged_signs(uint64_t seed, int n_heads, int dim, uint32_t *words) {
   for (int h = 0; h < n_heads; ++h) // head seeds as adaptq_mha_create gives them (upstream core/adaptq_c_api.cpp:160)
     aq_sign_words(seed ^ ((uint64_t)h * 0xDEADBEEFCAFEULL), P, words + (size_t)h * (P / 32), P / 32);
   return 0;
+}
+
+int adaptq_paged_take_status(const adaptq_paged_t *cache, int *taken, void *stream) {
+  const char *fn = "adaptq_paged_take_status";
+  aq_clear_error();
+  PagedView v;
+  if (!check_cache(fn, cache, v)) return -1;
+  if (!taken) return fail(fn, "null pointer"), -1;
+  if (misaligned(4, taken)) return fail(fn, "a pointer is not aligned to its elements"), -1;
+  DeviceScope dev(cache->device);
+  if (!dev.ok) return fail(fn, "no usable CUDA device (this library has no CPU path)"), -1;
+  take_status_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(v.status, taken);
+  return launched(fn) ? 0 : -1;
 }
 
 int adaptq_paged_append(const adaptq_paged_t *cache, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,

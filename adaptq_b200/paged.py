@@ -211,11 +211,15 @@ class PagedKVCache:
         return k, v
 
     def check(self):
-        """Wait for the device and raise RuntimeError if a call since the last check named a page outside the pool, or a
-        position or length without room in its block table (those entries were skipped)."""
-        status = int(self._status)
+        """Wait for the device -- all of its streams -- and raise RuntimeError if a call since the last check named a page
+        outside the pool, or a position or length without room in its block table (those entries were skipped).  Calls that
+        other threads make meanwhile report here or at the next check."""
+        torch.cuda.synchronize(self.device)
+        taken = torch.empty(1, dtype=torch.int32, device=self.device)
+        if self._L.adaptq_paged_take_status(self._ref, taken.data_ptr(), current_stream(self._index)):
+            raise RuntimeError(_lib.last_error())
+        status = int(taken)
         if status:
-            self._status.zero_()
             raise RuntimeError("PagedKVCache: " + "; ".join(text for bit, text in _STATUS if status & bit))
 
     @property

@@ -17,7 +17,8 @@
  * Values that only the device knows are checked there: an entry that would leave the
  * pool or the table is skipped and leaves a bit in *status -- 1: a page number outside the
  * pool, 2: a position or length that the block table has no room for.  The caller zeroes the
- * word and reads it when it likes.
+ * word at first; adaptq_paged_take_status() reads and zeroes it in one step, beside whatever
+ * calls are under way.
  */
 #ifndef ADAPTQ_PAGED_H
 #define ADAPTQ_PAGED_H
@@ -60,6 +61,10 @@ int adaptq_rotary_apply(const adaptq_rotary_t *rotary, const void *x, int64_t x_
 /* The sign words that adaptq_mha_create gives the heads of a handle with this seed.
  * words: HOST memory, [n_heads][padded / 32]. */
 int adaptq_paged_signs(uint64_t seed, int n_heads, int dim, uint32_t *words);
+
+/* *taken = *status, *status = 0, in one step and in the order of `stream`: bits that calls on
+ * other streams set are in this result or in the next. */
+int adaptq_paged_take_status(const adaptq_paged_t *cache, int *taken, void *stream);
 
 /* Append.  Tokens cu_tokens[b] .. cu_tokens[b+1]-1 of k and v ([n_tokens][n_kv_heads][dim])
  * belong to sequence b and take its positions starts[b] + start_bias and following; without

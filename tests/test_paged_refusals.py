@@ -95,3 +95,13 @@ def test_signs_are_those_of_the_rings(lib):
             assert (got == want).all()
     assert lib.adaptq_paged_signs(C.c_uint64(1), 1, 32, words.ctypes.data) == -1
     assert lib.adaptq_paged_signs(C.c_uint64(1), 1, 64, None) == -1
+
+
+def test_take_status_refusals(lib):
+    err = lambda: lib.adaptq_last_error().decode()  # noqa: E731
+    d = desc()
+    assert lib.adaptq_paged_take_status(None, 4096, None) == -1 and "null cache" in err()
+    assert lib.adaptq_paged_take_status(C.addressof(d), None, None) == -1 and "null pointer" in err()
+    assert lib.adaptq_paged_take_status(C.addressof(d), 4098, None) == -1 and "aligned" in err()
+    d = desc(status=None)
+    assert lib.adaptq_paged_take_status(C.addressof(d), 4096, None) == -1 and "null pointer" in err()
