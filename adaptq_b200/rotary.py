@@ -10,6 +10,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -20,6 +21,11 @@ try:  # the handle of the current stream without a Stream object around it: 2 us
 except AttributeError:
     def current_stream(index):
         return torch.cuda.current_stream(index).cuda_stream
+
+
+def _has_tangent(x):
+    """Whether x carries a forward-mode derivative (looked up only inside a dual level, where the module tells)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(x).tangent is not None
 
 
 def _inverse_frequencies(dim, base, scaling):
@@ -112,10 +118,10 @@ class Rotary:
     def __call__(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor = None) -> torch.Tensor:
         """x [tokens, heads, dim >= self.dim] (float32, float16 or bfloat16; any strides, the last one 1), positions
         [tokens] (int32 or int64) -> the same shape and type.  `out` may be x (in place).  Differentiable in x (without
-        `out`)."""
-        if x.requires_grad and torch.is_grad_enabled():
+        `out`), backwards and forwards."""
+        if (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x):
             if out is not None:
-                raise ValueError("out cannot be given for an x that requires a gradient")
+                raise ValueError("out cannot be given for an x that requires a gradient or has a tangent")
             return _Rotate.apply(x, positions, self)
         return self._apply(x.detach(), positions, out, 0)
 
@@ -153,11 +159,17 @@ class _Rotate(torch.autograd.Function):
     def forward(ctx, x, positions, rotary, inverse=0):
         ctx.rotary, ctx.inverse = rotary, inverse
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         return rotary._apply(x, positions, None, inverse)
 
     @staticmethod
     def backward(ctx, grad):
         positions, = ctx.saved_tensors
-        if grad.requires_grad and torch.is_grad_enabled():  # a gradient of the gradient is wanted: rotations all the way
+        if (grad.requires_grad and torch.is_grad_enabled()) or _has_tangent(grad):  # a derivative of the gradient is wanted
             return _Rotate.apply(grad, positions, ctx.rotary, 1 - ctx.inverse), None, None, None
         return ctx.rotary._apply(grad, positions, None, 1 - ctx.inverse), None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):  # the rotation is linear: the tangent turns as x does
+        positions, = ctx.saved_tensors
+        return _Rotate.apply(tangent, positions, ctx.rotary, ctx.inverse)

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from test_gpu_paged import ints, make_cache
+import paged_reference as ref
+from test_gpu_paged import BF16, F32, SCALINGS, ints, make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +42,43 @@ def test_status_is_taken_in_one_step(gen, gpu_lib):
         assert int(taken) == word and int(cache._status) == 0
     assert gpu_lib.adaptq_paged_take_status(cache._ref, None, None) == -1 and b"null" in gpu_lib.adaptq_last_error()
     assert gpu_lib.adaptq_paged_take_status(None, taken.data_ptr(), None) == -1 and b"null" in gpu_lib.adaptq_last_error()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_forward_mode_derivative(gen, dtype):
+    """The tangent of a rotation is the rotated tangent."""
+    from torch.autograd import forward_ad
+    from adaptq_b200 import Rotary
+    r = Rotary(24, scaling=SCALINGS[3])
+    x, dx = (torch.randn(5, 2, 40, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    pos = torch.arange(3, 8, device="cuda")
+    with forward_ad.dual_level():
+        y = r(forward_ad.make_dual(x, dx), pos)
+        primal, tangent = forward_ad.unpack_dual(y)
+        assert tangent is not None and torch.equal(tangent, r(dx, pos)) and torch.equal(primal, r(x, pos))
+        leaf = x.clone().requires_grad_()   # both directions at once
+        y = r(forward_ad.make_dual(leaf, dx), pos)
+        assert torch.equal(forward_ad.unpack_dual(y).tangent, r(dx, pos))
+        (g,) = torch.autograd.grad(forward_ad.unpack_dual(y).primal.float().sum(), leaf)
+        slope = dx.clone().requires_grad_()  # the tangent has a gradient of its own
+        y = r(forward_ad.make_dual(x, slope), pos)
+        (h,) = torch.autograd.grad(forward_ad.unpack_dual(y).tangent.float().sum(), slope)
+        assert torch.equal(g, h)
+        with pytest.raises(ValueError):
+            r(forward_ad.make_dual(x, dx), pos, out=torch.empty_like(x))
+        assert forward_ad.unpack_dual(r(x, pos)).tangent is None
+
+
+def test_forward_over_reverse(gen):
+    """The tangent of a gradient: of (c / 2) (R x)^2 it is R^T (c R dx)."""
+    from torch.autograd import forward_ad
+    from adaptq_b200 import Rotary
+    r, pos = Rotary(24, scaling=SCALINGS[3]), torch.arange(3, 8, device="cuda")
+    x, dx, c = (torch.randn(5, 2, 40, generator=gen, device="cuda") for _ in range(3))
+    x.requires_grad_()
+    with forward_ad.dual_level():
+        y = r(forward_ad.make_dual(x, dx), pos)
+        (g,) = torch.autograd.grad((y * y * c).sum() / 2, x, create_graph=True)
+        tangent = forward_ad.unpack_dual(g).tangent
+    want = ref.rotate(c.double() * ref.rotate(dx.double(), pos, r), pos, r, inverse=True)
+    assert tangent is not None and float((tangent.double() - want).abs().max()) <= 1e-5 * float(want.abs().max())
