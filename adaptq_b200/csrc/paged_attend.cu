@@ -20,7 +20,7 @@ static int sm_count(int device) {
 }
 
 // The names below are the same in every unit: what differs between units carries the bit widths in its type.
-struct AttendRoom { size_t query_scales, block_headers, block_slots, warp_slots, total; }; // offsets in the workspace
+struct AttendRoom { size_t query_scales, block_headers, block_slots, warp_slots, warp_sums, total; }; // offsets in the workspace
 
 template <typename S> static AttendRoom attend_room(int blocks, int cols, size_t items) {
   const size_t slot = (size_t)cols * (S::DIM + 4) * sizeof(float);
@@ -29,7 +29,8 @@ template <typename S> static AttendRoom attend_room(int blocks, int cols, size_t
   r.block_headers = r.query_scales + items * 32;
   r.block_slots = r.block_headers + (size_t)blocks * sizeof(int4);
   r.warp_slots = r.block_slots + blocks * 2 * slot;
-  r.total = r.warp_slots + (size_t)blocks * S::WARPS * 2 * slot;
+  r.warp_sums = r.warp_slots + (size_t)blocks * S::WARPS * 2 * slot;
+  r.total = r.warp_sums + (size_t)blocks * S::WARPS * S::SUMS * sizeof(float);
   return r;
 }
 
@@ -59,6 +60,7 @@ template <typename S> static bool launch_attend(const AttendCall &call) {
   a.block_headers = reinterpret_cast<int4 *>(base + room.block_headers);
   a.block_slots = reinterpret_cast<float *>(base + room.block_slots);
   a.warp_slots = reinterpret_cast<float *>(base + room.warp_slots);
+  a.warp_sums = reinterpret_cast<float *>(base + room.warp_sums);
   paged_query_kernel<S::DIM><<<(unsigned)items, QUERY_WARPS * 32, 0, call.stream>>>(
       a, S::COLS, 1.4426950408889634f / (S::DIM * table_scale(S::KEY_BITS)));
   if (!aq_launched(fn)) return false;

@@ -16,11 +16,12 @@ struct AttendLaunch {
   int n_seqs, group, passes, type;
   float scale;
   int q_vec, out_vec;
-  // workspace: the queries as operands and their scales, a header per block, the blocks' partial results, the warps'
+  // workspace: the queries as operands and their scales, a header per block, the blocks' partial results, the warps', the
+  // warps' sums under way
   uint32_t *operands; // [item][P / 8][32]
   float *query_scales; // [item][8]
   int4 *block_headers;
-  float *block_slots, *warp_slots;
+  float *block_slots, *warp_slots, *warp_sums;
   int slot_cols; // columns of a partial result
 };
 

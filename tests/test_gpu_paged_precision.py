@@ -32,3 +32,41 @@ def test_sums_over_long_runs(gen, dtype, kb, vb, dim):
     got = cache.attend(q.expand(seqs, -1, -1), table, torch.full((seqs,), n, dtype=torch.int32, device="cuda"))
     cache.check()
     attend_close(got, want.expand(seqs, -1, -1), dtype)
+
+
+@pytest.mark.parametrize("dtype,kb,vb,dim,n,cuts", [(F16, 4, 4, 128, 131072, "even"), (F16, 3, 2, 128, 131072, "even"), (F16, 2, 3, 64, 131072, "even"),
+                                                    (F16, 4, 2, 256, 65536, "even"), (F16, 4, 4, 128, 131072, "ragged")])
+def test_sums_of_16_bit_calls_over_long_runs(gen, dtype, kb, vb, dim, n, cuts):
+    """As above, by how far the output is off along its own direction, where errors of one sign show and the output's
+    rounding (known from the definition) mostly cancels.  The tensor cores cut 2^-23 off a sum at every product and hand
+    it over after 256 of them: 2^-15.  The codebook of 4 bits moves the row of values by 7.8e-5 of itself at random
+    (3 sigma over its coordinates: 2.1e-5 at 128), the other two by less.  A shift of up to 5.2e-5 crosses a border of
+    the output's rounding, 2^-11 of the value apart at least, for a share of 0.11 of the outputs at random: 3 sigma over
+    them are 3 sqrt(0.11 / 128) 2^-11 = 4.3e-5 along it.  1e-4 in all."""
+    seqs, page = 148 * 16, 256
+    cache, signs = make_cache(gen, n // page, 1, dim, kb, vb, page)
+    ref.random_pool(cache, gen)
+    cache.v_pages[:] = cache.v_pages[0, 0, 0]
+    cache.v_scales.fill_(1.375)
+    table = torch.randperm(n // page, generator=gen, device="cuda").int()[None].expand(seqs, -1)
+    if cuts == "even":
+        lengths = torch.full((seqs,), n, dtype=torch.int32, device="cuda")
+    else:   # empty and shorter sequences between the others
+        lengths = torch.randint(0, n + 1, (seqs,), generator=gen, device="cuda", dtype=torch.int32)
+        lengths[::7] = 0
+        lengths[1::7] = n
+    q = torch.randn(1, 1, dim, generator=gen, device="cuda").to(dtype)
+    want = ref.attend(cache, signs, q, table[:1], ints(n))[0, 0]   # one row, whatever the weights and the length
+    got = cache.attend(q.expand(seqs, -1, -1), table, lengths)[:, 0]
+    cache.check()
+    along = lambda y: (y.double() @ want) / (want @ want)  # noqa: E731
+    off = (along(got) - along(want.to(dtype)))[lengths > 0].abs()
+    assert float(off.max()) <= 1e-4 * max(1.0, math.sqrt(128 / dim)), float(off.max())
+    assert not got[lengths == 0].any()
+    # the reference of the exponentials moves while sums lie in the workspace: weights that grow along the sequence
+    if cuts == "even":
+        cache.v_scales.copy_(1.375 * torch.exp2(24.0 * (torch.arange(n, device="cuda") - n) / n)[torch.argsort(table[0])[:, None] * page + torch.arange(page, device="cuda")][:, None])
+        want = ref.attend(cache, signs, q, table[:1], ints(n))[0, 0]
+        got = cache.attend(q.expand(seqs, -1, -1), table, lengths)[:, 0]
+        off = (along(got) - along(want.to(dtype))).abs()
+        assert float(off.max()) <= 1e-4 * max(1.0, math.sqrt(128 / dim)), float(off.max())
