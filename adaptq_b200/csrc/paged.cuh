@@ -32,13 +32,16 @@ struct TableView {
 };
 
 // cos and sin of position * w, times the factor.  The frequency is a 64-bit binary fraction of
-// a turn, so the product modulo 2^64 is the phase modulo one turn, exact at every position;
-// only its last rounding, to 24 bits of half a turn, is left (1e-7 absolute in the angle).
+// a turn, so the product modulo 2^64 is the phase modulo one turn, exact at every position.
+// The nearest quarter turn is taken off in integers: of the eighth of a turn at most that is
+// left, rounding to 24 bits takes 2e-8, and nothing that counts next to a zero of either.
 __device__ __forceinline__ float2 rotary_turn(const RotaryView &r, int pair, long long pos) {
-  const long long phase = (long long)((unsigned long long)pos * r.turns[pair]);
+  const unsigned long long phase = (unsigned long long)pos * r.turns[pair];
+  const unsigned quarter = (unsigned)((phase + (1ull << 61)) >> 62);
   float s, c;
-  sincospif((float)phase * 0x1p-63f, &s, &c); // phase / 2^63 half turns, in [-1, 1)
-  return make_float2(c * r.factor, s * r.factor);
+  sincospif((float)(long long)(phase - ((unsigned long long)quarter << 62)) * 0x1p-63f, &s, &c); // in half turns, from -1/4 to 1/4
+  const float x = (quarter & 1) ? -s : c, y = (quarter & 1) ? c : s;
+  return (quarter & 2) ? make_float2(-x * r.factor, -y * r.factor) : make_float2(x * r.factor, y * r.factor);
 }
 
 // One element of a rotated pair: mine * cos -+ other * sin (minus for the pair's first element).  One order of

@@ -81,4 +81,4 @@ def test_forward_over_reverse(gen):
         (g,) = torch.autograd.grad((y * y * c).sum() / 2, x, create_graph=True)
         tangent = forward_ad.unpack_dual(g).tangent
     want = ref.rotate(c.double() * ref.rotate(dx.double(), pos, r), pos, r, inverse=True)
-    assert tangent is not None and float((tangent.double() - want).abs().max()) <= 1e-5 * float(want.abs().max())
+    assert tangent is not None and float((tangent.detach().double() - want.detach()).abs().max()) <= 1e-5 * float(want.detach().abs().max())

@@ -70,3 +70,30 @@ def test_sums_of_16_bit_calls_over_long_runs(gen, dtype, kb, vb, dim, n, cuts):
         got = cache.attend(q.expand(seqs, -1, -1), table, lengths)[:, 0]
         off = (along(got) - along(want.to(dtype))).abs()
         assert float(off.max()) <= 1e-4 * max(1.0, math.sqrt(128 / dim)), float(off.max())
+
+
+def test_phases_are_exact_to_float32():
+    """The phase is reduced to an eighth of a turn in integers before it is rounded to 24 bits, so cosine and sine are
+    off by 2^-24 of themselves from that rounding and by 2^-23 (one step) each from the functions: below 2^-22 of the
+    value wherever it is, next to a zero crossing as well."""
+    from adaptq_b200 import Rotary
+    r = Rotary(64, 10000.0)
+    gen = torch.Generator().manual_seed(3)
+    pos = torch.randint(0, 2 ** 40, (4000,), generator=gen)
+    pos[0], pos[1] = 0, 1
+    x = torch.zeros(4000, 1, 64, device="cuda")
+    x[..., :32] = 1.0
+    y = r(x, pos.cuda()).double().cpu()[:, 0]
+    c = np.empty((4000, 32))
+    s = np.empty((4000, 32))
+    for j, w in enumerate(int(t) % 2 ** 64 for t in r._turns.cpu().tolist()):
+        for i, p in enumerate(pos.tolist()):
+            phase = (p * w) % 2 ** 64
+            quarter = (phase + 2 ** 61) >> 62
+            a = (phase - (quarter << 62)) / 2.0 ** 64 * 2 * math.pi
+            c[i, j], s[i, j] = [(math.cos(a), math.sin(a)), (-math.sin(a), math.cos(a)), (-math.cos(a), -math.sin(a)), (math.sin(a), -math.cos(a))][quarter % 4]
+    for got, want in ((y[:, :32], c), (y[:, 32:], s)):
+        want = torch.from_numpy(want)
+        assert float(want.abs().min()) < 1e-4   # zero crossings are among them
+        err = ((got - want).abs() - 2.0 ** -22 * want.abs()).max()
+        assert float(err) <= 1e-30, float(err)
