@@ -72,7 +72,8 @@ template <int P> __device__ __forceinline__ void row_butterflies(float2 (&x)[16]
   }
 }
 
-// Quantisers.  2 bits: evenly spaced thresholds, one rounding.  3 and 4 bits: the 128 buckets of a quarter from -16 on hold at most one threshold each, so a code is the
+// Quantisers: a code is the count of thresholds at or below the coordinate.  2 bits: evenly spaced thresholds, one
+// rounding.  3 and 4 bits: the 128 buckets of a quarter from -16 on hold at most one threshold each, so a code is the
 // count of thresholds at or below the bucket's start and one comparison.  16 copies of the table, entry by entry, keep the
 // half-warps of a 64-bit read apart.  A coordinate is at most sqrt(P) = 16 in size.
 constexpr int BUCKETS = 128, BUCKET_COPIES = 16;
@@ -92,9 +93,10 @@ template <int BITS> __device__ __forceinline__ void fill_buckets(uint2 *table, i
 // word = word << BITS | code of u
 template <int P, int BITS> __device__ __forceinline__ void push_code(uint32_t &word, float u, const uint2 *table, uint32_t copy /* 8 * lane's copy */) {
   if constexpr (BITS == 2) {
-    // thresholds -T, 0, T: the code is floor(u / T) + 2 within 0 .. 3
+    // thresholds -T, 0, T: the code is floor(u / T) + 2 within 0 .. 3.  T * (1 / T) rounds to less than one, which
+    // is right at -T (a threshold counts from itself on) and would be wrong at T: that one is a comparison.
     constexpr float T = (0.4528f + 1.5104f) * 0.5f;
-    const float v = fminf(fmaxf(u, -1.5f * T), 1.5f * T);
+    const float v = u >= T ? 1.5f * T : fmaxf(u, -1.5f * T);
     word = word * 4 + (__float_as_uint(__fmaf_rd(v, 1.f / T, 8388608.f + 2.f)) & 3u);
   } else {
     if constexpr (P == 256) u = fminf(fmaxf(u, -16.f), 15.75f);

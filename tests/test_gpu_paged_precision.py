@@ -97,3 +97,40 @@ def test_phases_are_exact_to_float32():
         assert float(want.abs().min()) < 1e-4   # zero crossings are among them
         err = ((got - want).abs() - 2.0 ** -22 * want.abs()).max()
         assert float(err) <= 1e-30, float(err)
+
+
+@pytest.mark.parametrize("bits", [2, 3, 4])
+def test_coordinates_at_a_threshold(gen, bits):
+    """A code counts the thresholds at or below its coordinate: (a, b, 0, ...) has the coordinates (a +- b) / norm, and
+    pairs are searched (float32, rounded operation by operation as the kernel does it) that give a threshold exactly."""
+    from adaptq_b200 import PagedKVCache
+    f = np.float32
+    m = [f(v) for v in ref.MAGNITUDES[bits]]
+    level = [-v for v in reversed(m)] + m
+    thresholds = [(p + q) * f(0.5) for p, q in zip(level, level[1:])]
+    rng = np.random.default_rng(bits)
+    rows, want = [], []
+    for t in thresholds:
+        if abs(t) >= math.sqrt(2):
+            continue
+        size, sign = abs(t), f(-1 if t < 0 else 1)
+        found = 0
+        for a in rng.uniform(1, 2, 200).astype(f):
+            b = f(a * math.tan(math.asin(float(size) / math.sqrt(2)) - math.pi / 4))
+            bb = next((c for c in (f(b + f(k) * np.spacing(b)) for k in range(-3, 4))
+                       if f(f(a + c) * (f(1) / np.sqrt(f(f(f(a * a) + f(c * c)) + f(1e-12))))) == size), None)
+            if bb is not None and found < 4:
+                other = sign * f(f(a - bb) * (f(1) / np.sqrt(f(f(f(a * a) + f(bb * bb)) + f(1e-12)))))
+                rows.append((sign * a, sign * bb))
+                want.append((sum(x <= t for x in thresholds), sum(x <= other for x in thresholds)))
+                found += 1
+        assert found == 4
+    n = len(rows)
+    x = torch.zeros(n, 1, 64)
+    x[:, 0, :2] = torch.from_numpy(np.array(rows, np.float32))
+    cache = PagedKVCache(1, 1, 64, bits, bits, 64, signs=torch.ones(1, 64))
+    cache.append(x.cuda(), x.cuda(), ints(0).view(1, 1), ints(0), ints(0, n))
+    for pages in (cache.k_pages, cache.v_pages):
+        code = ref.unpack(pages[0, 0, :n], bits).cpu()
+        expect = torch.tensor(want)
+        assert torch.equal(code[:, ::2], expect[:, :1].expand(n, 32)) and torch.equal(code[:, 1::2], expect[:, 1:].expand(n, 32))
