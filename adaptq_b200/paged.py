@@ -14,7 +14,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .rotary import TYPES, Rotary, current_stream
+from .rotary import TYPES, Rotary, check_written, current_stream, increment_version
 
 _STATUS = ((1, "a block table names a page outside the pool"), (2, "a position or length has no room in its block table"))
 
@@ -152,7 +152,8 @@ class PagedKVCache:
     def attend(self, q, block_table, lengths, rotary=None, scale=None, out=None):
         """Attention of one token per sequence over its first lengths[b] tokens.  q: (sequences, query heads, dim), query head
         j reading KV head j // (query heads / KV heads) -> the same shape and type.  Queries are rotated by position
-        lengths[b] - 1 first, if `rotary`.  scale: 1/sqrt(dim) by default.  A sequence of length 0 gives zeros."""
+        lengths[b] - 1 first, if `rotary`.  scale: 1/sqrt(dim) by default.  A sequence of length 0 gives zeros.  `out` may be
+        q and is marked as modified; no gradient flows through."""
         if q.dim() != 3 or q.shape[2] != self.dim or q.shape[1] % self.n_kv_heads or not q.shape[1] or q.dtype not in TYPES or q.get_device() != self._index:
             raise ValueError(f"q must be (sequences, a multiple of {self.n_kv_heads} heads, {self.dim}) float32, float16 or bfloat16 on {self.device}, "
                              f"got {tuple(q.shape)} {q.dtype} on {q.device}")
@@ -162,10 +163,13 @@ class PagedKVCache:
         if table.shape[0] != n:
             raise ValueError(f"block_table has {table.shape[0]} sequences, q {n}")
         lengths = self._ints("lengths", lengths, n)
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty((n, heads, self.dim), dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
             raise ValueError("out must have the shape, type and device of q and contiguous rows")
+        else:
+            check_written("out", out)
         kind = TYPES[q.dtype]
         size = self._sizes.get((n, heads, kind))
         if size is None:
@@ -178,6 +182,8 @@ class PagedKVCache:
                                        self._scale if scale is None else float(scale), self._rotary(rotary), workspace.data_ptr(), size,
                                        current_stream(self._index)):
             raise RuntimeError(_lib.last_error())
+        if given:
+            increment_version(out)
         return out
 
     def step(self, k, v, q, block_table, lengths, rotary=None, scale=None, out=None):
@@ -204,10 +210,16 @@ class PagedKVCache:
             self._rows("out[1]", v, self.n_kv_heads)
             if k.shape[0] != total or v.shape != k.shape or v.dtype != k.dtype or k.stride(2) != 1 or v.stride(2) != 1:
                 raise ValueError(f"out must be two tensors of {total} rows, of one type, with contiguous rows")
+            check_written("out[0]", k)
+            check_written("out[1]", v)
+            if total and k.data_ptr() == v.data_ptr():
+                raise ValueError("out must be two tensors, not one twice")
         ks, vs = k.stride(), v.stride()
         if self._L.adaptq_paged_read(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], TYPES[k.dtype], table.data_ptr(),
                                      table.stride(0), table.shape[1], starts.data_ptr(), cu_tokens.data_ptr(), n_seqs, int(total), current_stream(self._index)):
             raise RuntimeError(_lib.last_error())
+        if out is not None:
+            increment_version((k, v))
         return k, v
 
     def check(self):

@@ -11,6 +11,7 @@ import math
 import numpy as np
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -26,6 +27,15 @@ except AttributeError:
 def _has_tangent(x):
     """Whether x carries a forward-mode derivative (looked up only inside a dual level, where the module tells)."""
     return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(x).tangent is not None
+
+
+def check_written(name, t):
+    """Refuse a (n, heads, dim) tensor with contiguous rows as an output if autograd follows it or its rows overlap."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} cannot be a tensor that requires a gradient")
+    n, heads, dim = t.shape
+    if (n > 1 and abs(t.stride(0)) < dim) or (heads > 1 and abs(t.stride(1)) < dim):
+        raise ValueError(f"the rows of {name} overlap: shape {tuple(t.shape)}, strides {t.stride()}")
 
 
 def _inverse_frequencies(dim, base, scaling):
@@ -118,7 +128,7 @@ class Rotary:
     def __call__(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor = None) -> torch.Tensor:
         """x [tokens, heads, dim >= self.dim] (float32, float16 or bfloat16; any strides, the last one 1), positions
         [tokens] (int32 or int64) -> the same shape and type.  `out` may be x (in place).  Differentiable in x (without
-        `out`), backwards and forwards."""
+        `out`), backwards and forwards.  A given `out` is marked as modified, as PyTorch's own in-place operations do."""
         if (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x):
             if out is not None:
                 raise ValueError("out cannot be given for an x that requires a gradient or has a tangent")
@@ -141,16 +151,21 @@ class Rotary:
         if xs[2] != 1 and dim > 1:
             x = x.contiguous()
             xs = x.stride()
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty((n, heads, dim), dtype=x.dtype, device=self.device)
         elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (dim > 1 and out.stride(2) != 1):
             raise ValueError("out must have the shape, type and device of x and contiguous rows")
+        else:
+            check_written("out", out)
         if not positions.is_contiguous():
             positions = positions.contiguous()
         ys = out.stride()
         if self._L.adaptq_rotary_apply(self._ref, x.data_ptr(), xs[0], xs[1], out.data_ptr(), ys[0], ys[1], kind, positions.data_ptr(), wide,
                                        n, heads, dim, inverse, self._index, current_stream(self._index)):
             raise RuntimeError(_lib.last_error())
+        if given:
+            increment_version(out)
         return out
 
 

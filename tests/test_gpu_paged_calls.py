@@ -82,3 +82,54 @@ def test_forward_over_reverse(gen):
         tangent = forward_ad.unpack_dual(g).tangent
     want = ref.rotate(c.double() * ref.rotate(dx.double(), pos, r), pos, r, inverse=True)
     assert tangent is not None and float((tangent.detach().double() - want.detach()).abs().max()) <= 1e-5 * float(want.detach().abs().max())
+
+
+def test_tensors_written_in_place_are_marked(gen):
+    """A tensor that a backward pass still needs cannot be overwritten unnoticed."""
+    from adaptq_b200 import Rotary
+    r, pos = Rotary(64), torch.arange(3, device="cuda")
+    cache, _ = make_cache(gen, 4, 2, 64, 4, 4, 16)
+    ref.random_pool(cache, gen)
+    table, n = ints(0, 1, 2).view(3, 1), ints(5, 6, 7)
+    q = torch.randn(3, 2, 64, generator=gen, device="cuda")
+    calls = [lambda o: r(q, pos, out=o), lambda o: r(o, pos, out=o), lambda o: cache.attend(q, table, n, out=o),
+             lambda o: cache.read(table, ints(0, 0, 0), ints(0, 1, 2, 3), 3, out=(o, torch.empty_like(o))),
+             lambda o: cache.read(table, ints(0, 0, 0), ints(0, 1, 2, 3), 3, out=(torch.empty_like(o), o)),
+             lambda o: cache.step(q, q, q, table, n, out=o)]
+    for call in calls:
+        w = torch.ones(3, 2, 64, device="cuda", requires_grad=True)
+        saved = torch.randn(3, 2, 64, generator=gen, device="cuda")
+        y = (w * saved).sum()
+        call(saved)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with pytest.raises(ValueError, match="gradient"):
+            call(torch.zeros(3, 2, 64, device="cuda", requires_grad=True))
+        with torch.no_grad():
+            call(torch.zeros(3, 2, 64, device="cuda", requires_grad=True))
+        with torch.inference_mode():
+            call(torch.zeros(3, 2, 64, device="cuda"))
+
+
+def test_outputs_whose_rows_overlap_are_refused(gen):
+    from adaptq_b200 import Rotary
+    r, pos = Rotary(64), torch.arange(3, device="cuda")
+    cache, _ = make_cache(gen, 4, 2, 64, 4, 4, 16)
+    ref.random_pool(cache, gen)
+    table, n = ints(0, 1, 2).view(3, 1), ints(5, 6, 7)
+    x = torch.randn(3, 2, 64, generator=gen, device="cuda")
+    flat = torch.zeros(4096, device="cuda")
+    for bad in (flat[:64].expand(3, 2, 64), flat[:128].view(1, 2, 64).expand(3, 2, 64), flat[:192].view(3, 1, 64).expand(3, 2, 64),
+                flat.as_strided((3, 2, 64), (128, 63, 1)), flat.as_strided((3, 2, 64), (32, 512, 1))):
+        for call in (lambda: r(x, pos, out=bad), lambda: cache.attend(x, table, n, out=bad),
+                     lambda: cache.read(table, ints(0, 0, 0), ints(0, 1, 2, 3), 3, out=(bad, x.clone())),
+                     lambda: cache.read(table, ints(0, 0, 0), ints(0, 1, 2, 3), 3, out=(x.clone(), bad))):
+            with pytest.raises(ValueError, match="overlap"):
+                call()
+    with pytest.raises(ValueError, match="one twice"):
+        cache.read(table, ints(0, 0, 0), ints(0, 1, 2, 3), 3, out=(x, x))
+    assert not flat.any()
+    want, one = r(x, pos), r(x[:1], pos[:1])
+    for good in (flat[:384].view(2, 3, 64).transpose(0, 1), flat.as_strided((3, 2, 64), (200, 1000, 1))):
+        assert torch.equal(r(x, pos, out=good), want)
+    assert torch.equal(r(x[:1], pos[:1], out=flat.as_strided((1, 2, 64), (0, 64, 1))), one)
