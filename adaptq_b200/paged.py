@@ -9,6 +9,7 @@ ordered.
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import numpy as np
 import torch
@@ -154,6 +155,9 @@ class PagedKVCache:
         j reading KV head j // (query heads / KV heads) -> the same shape and type.  Queries are rotated by position
         lengths[b] - 1 first, if `rotary`.  scale: 1/sqrt(dim) by default.  A sequence of length 0 gives zeros.  `out` may be
         q and is marked as modified; no gradient flows through."""
+        return self._attend(*self._attend_arguments(q, block_table, lengths, rotary, scale, out))
+
+    def _attend_arguments(self, q, block_table, lengths, rotary, scale, out):
         if q.dim() != 3 or q.shape[2] != self.dim or q.shape[1] % self.n_kv_heads or not q.shape[1] or q.dtype not in TYPES or q.get_device() != self._index:
             raise ValueError(f"q must be (sequences, a multiple of {self.n_kv_heads} heads, {self.dim}) float32, float16 or bfloat16 on {self.device}, "
                              f"got {tuple(q.shape)} {q.dtype} on {q.device}")
@@ -170,6 +174,13 @@ class PagedKVCache:
             raise ValueError("out must have the shape, type and device of q and contiguous rows")
         else:
             check_written("out", out)
+        scale = self._scale if scale is None else C.c_float(scale).value
+        if not 0.0 < scale < math.inf:
+            raise RuntimeError(f"scale must be positive and finite, got {scale}")
+        return q, table, lengths, self._rotary(rotary), scale, out, given
+
+    def _attend(self, q, table, lengths, rotary, scale, out, given):
+        n, heads = q.shape[0], q.shape[1]
         kind = TYPES[q.dtype]
         size = self._sizes.get((n, heads, kind))
         if size is None:
@@ -179,8 +190,7 @@ class PagedKVCache:
         qs, os = q.stride(), out.stride()
         if self._L.adaptq_paged_attend(self._ref, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], kind, table.data_ptr(),
                                        table.stride(0), table.shape[1], lengths.data_ptr(), n, heads,
-                                       self._scale if scale is None else float(scale), self._rotary(rotary), workspace.data_ptr(), size,
-                                       current_stream(self._index)):
+                                       scale, rotary, workspace.data_ptr(), size, current_stream(self._index)):
             raise RuntimeError(_lib.last_error())
         if given:
             increment_version(out)
@@ -188,9 +198,11 @@ class PagedKVCache:
 
     def step(self, k, v, q, block_table, lengths, rotary=None, scale=None, out=None):
         """One decode step: the new token of every sequence enters as its last (position lengths[b] - 1: lengths count it),
-        then its queries attend.  k, v (sequences, heads, dim), q as for attend; a sequence of length 0 takes no part."""
+        then its queries attend.  k, v (sequences, heads, dim), q as for attend; a sequence of length 0 takes no part.
+        Arguments that are refused leave the cache as it was."""
+        arguments = self._attend_arguments(q, block_table, lengths, rotary, scale, out)
         self._append(k, v, block_table, lengths, -1, None, rotary)
-        return self.attend(q, block_table, lengths, rotary=rotary, scale=scale, out=out)
+        return self._attend(*arguments)
 
     def read(self, block_table, starts, cu_tokens, total, dtype=torch.bfloat16, out=None):
         """Tokens back as rows: (k, v), each (total, heads, dim) of `dtype`, keys as stored (rotated).  Sequence b gives its

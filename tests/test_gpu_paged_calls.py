@@ -133,3 +133,19 @@ def test_outputs_whose_rows_overlap_are_refused(gen):
     for good in (flat[:384].view(2, 3, 64).transpose(0, 1), flat.as_strided((3, 2, 64), (200, 1000, 1))):
         assert torch.equal(r(x, pos, out=good), want)
     assert torch.equal(r(x[:1], pos[:1], out=flat.as_strided((1, 2, 64), (0, 64, 1))), one)
+
+
+def test_refused_steps_store_nothing(gen):
+    cache, _ = make_cache(gen, 4, 2, 64, 4, 4, 16)
+    ref.random_pool(cache, gen)
+    before = [t.clone() for t in (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales)]
+    table, n = ints(0, 1, 2).view(3, 1), ints(5, 6, 7)
+    k, q = torch.randn(3, 2, 64, generator=gen, device="cuda"), torch.randn(3, 4, 64, generator=gen, device="cuda")
+    for bad in (lambda: cache.step(k, k, q[:, :3], table, n), lambda: cache.step(k, k, q[:2], table, n), lambda: cache.step(k, k, q.double(), table, n),
+                lambda: cache.step(k, k, q, table, n, out=q[:, :2]), lambda: cache.step(k, k, q, table, n, scale=0.0),
+                lambda: cache.step(k, k, q, table, n, scale=1e60), lambda: cache.step(k, k[:2], q, table, n), lambda: cache.step(k, k, q, table, n, rotary=1)):
+        with pytest.raises((ValueError, RuntimeError)):
+            bad()
+        assert all(torch.equal(a, b) for a, b in zip(before, (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales)))
+    cache.step(k, k, q, table, n)
+    assert not torch.equal(before[0], cache.k_pages)
