@@ -115,6 +115,7 @@ int rows_call(const char *fn, bool append, const adaptq_paged_t *cache, void *k,
   if (!k || !v || !table || !starts) return fail(fn, "null pointer"), -1;
   if (misaligned(size_of(type), k, v) || misaligned(4, table, starts, cu_tokens)) return fail(fn, "a pointer is not aligned to its elements"), -1;
   const int P = padded_of(cache->dim);
+  if (cu_tokens && n_seqs > 1 << 30) return fail(fn, "too many sequences for one call"), -1; // owner_of looks up to n_seqs + 32 ahead, in 32 bits
   if (n_tokens > (1ll << 31) / cache->n_kv_heads) return fail(fn, "too many tokens for one call"), -1;
   a.table = TableView{table, table_stride, table_width};
   a.starts = starts; a.start_bias = start_bias; a.cu = cu_tokens; a.n_seqs = n_seqs; a.n_tokens = n_tokens;
