@@ -258,7 +258,6 @@ int adaptq_paged_attend(const adaptq_paged_t *cache, const void *q, int64_t q_se
   a.lengths = lengths; a.q = q; a.out = out; a.q_seq = q_seq_stride; a.q_head = q_head_stride;
   a.out_seq = out_seq_stride; a.out_head = out_head_stride;
   a.n_seqs = n_seqs; a.group = n_q_heads / cache->n_kv_heads; a.type = type; a.scale = scale;
-  a.q_vec = vector_rows(q, q_seq_stride, q_head_stride, cache->dim, type);
   a.out_vec = vector_rows(out, out_seq_stride, out_head_stride, cache->dim, type);
   if (!workspace || !aligned(workspace, 16) || workspace_bytes < adaptq_paged_attend_workspace(cache, n_seqs, n_q_heads, type))
     return fail(fn, "the workspace is too small or not 16-byte aligned"), -1;

@@ -15,7 +15,7 @@ struct AttendLaunch {
   long long q_seq, q_head, out_seq, out_head;
   int n_seqs, group, passes, type;
   float scale;
-  int q_vec, out_vec;
+  int out_vec;
   // workspace: the queries as operands and their scales, a header per block, the blocks' partial results, the warps', the
   // warps' sums under way
   uint32_t *operands; // [item][P / 8][32]
