@@ -72,35 +72,35 @@ bool check_type(const char *fn, int type) { return type >= 0 && type <= 2 ? true
 
 bool launched(const char *fn) { return aq_launched(fn); }
 
-template <int P, int KB, int VB> void launch_rows(const RowsLaunch &a, bool append, cudaStream_t s) {
+template <int P, int KB, int VB> void launch_rows(const RowsLaunch &a, bool append, int sms, cudaStream_t s) {
   if (append) {
     constexpr int ROWS = rows_per_warp<P>, WARPS = ROWS_THREADS / 32;
     RowsLaunch b = a;
     b.turn_tokens = std::min(ROWS, (ROWS + a.c.heads - 2) / a.c.heads + 1);
     // several tokens a warp, since what it sets up is paid once, and three rounds of warps (24 an SM, keys and values), for
     // keys take longer than values
-    b.job_tokens = (int)std::max(1ll, std::min(32ll, 2 * a.n_tokens / (3 * 148 * 24)));
+    b.job_tokens = (int)std::max(1ll, std::min(32ll, 2 * a.n_tokens / (3 * 24 * sms)));
     const unsigned blocks = (unsigned)((a.n_tokens + b.job_tokens * WARPS - 1) / (b.job_tokens * WARPS));
     paged_append_kernel<P, KB, VB><<<dim3(blocks, 2), ROWS_THREADS, (size_t)WARPS * b.turn_tokens * a.r.dim * sizeof(float), s>>>(b);
   } else {
     RowsLaunch b = a;
-    // blocks of 64 tokens, smaller ones where those would leave SMs without work
-    for (b.block_tokens = READ_TOKENS; b.block_tokens > 16 && 2 * ((a.n_tokens + b.block_tokens - 1) / b.block_tokens) < 592;) b.block_tokens /= 2;
+    // blocks of 64 tokens (keys and values), smaller ones where those would not make four an SM
+    for (b.block_tokens = READ_TOKENS; b.block_tokens > 16 && 2 * ((a.n_tokens + b.block_tokens - 1) / b.block_tokens) < 4 * sms;) b.block_tokens /= 2;
     const unsigned tiles = (unsigned)((a.n_tokens + b.block_tokens - 1) / b.block_tokens);
     const long long items = (long long)(b.block_tokens / 16) * a.c.heads;
-    const unsigned shares = (unsigned)std::max(1ll, std::min((items + READ_WARPS - 1) / READ_WARPS, 592ll / (2 * tiles)));
+    const unsigned shares = (unsigned)std::max(1ll, std::min((items + READ_WARPS - 1) / READ_WARPS, 4ll * sms / (2 * tiles)));
     paged_read_kernel<P, KB, VB><<<dim3(tiles, 2, shares), READ_WARPS * 32, 0, s>>>(b);
   }
 }
-template <int P, int KB> void launch_rows_v(const RowsLaunch &a, int vb, bool append, cudaStream_t s) {
-  if (vb == 2) launch_rows<P, KB, 2>(a, append, s);
-  else if (vb == 3) launch_rows<P, KB, 3>(a, append, s);
-  else launch_rows<P, KB, 4>(a, append, s);
+template <int P, int KB> void launch_rows_v(const RowsLaunch &a, int vb, bool append, int sms, cudaStream_t s) {
+  if (vb == 2) launch_rows<P, KB, 2>(a, append, sms, s);
+  else if (vb == 3) launch_rows<P, KB, 3>(a, append, sms, s);
+  else launch_rows<P, KB, 4>(a, append, sms, s);
 }
-template <int P> void launch_rows_k(const RowsLaunch &a, int kb, int vb, bool append, cudaStream_t s) {
-  if (kb == 2) launch_rows_v<P, 2>(a, vb, append, s);
-  else if (kb == 3) launch_rows_v<P, 3>(a, vb, append, s);
-  else launch_rows_v<P, 4>(a, vb, append, s);
+template <int P> void launch_rows_k(const RowsLaunch &a, int kb, int vb, bool append, int sms, cudaStream_t s) {
+  if (kb == 2) launch_rows_v<P, 2>(a, vb, append, sms, s);
+  else if (kb == 3) launch_rows_v<P, 3>(a, vb, append, sms, s);
+  else launch_rows_v<P, 4>(a, vb, append, sms, s);
 }
 
 int rows_call(const char *fn, bool append, const adaptq_paged_t *cache, void *k, int64_t k_token, int64_t k_head, void *v,
@@ -129,9 +129,10 @@ int rows_call(const char *fn, bool append, const adaptq_paged_t *cache, void *k,
   DeviceScope dev(cache->device);
   if (!dev.ok) return fail(fn, "no usable CUDA device (this library has no CPU path)"), -1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (P == 64) launch_rows_k<64>(a, cache->k_bits, cache->v_bits, append, s);
-  else if (P == 128) launch_rows_k<128>(a, cache->k_bits, cache->v_bits, append, s);
-  else launch_rows_k<256>(a, cache->k_bits, cache->v_bits, append, s);
+  const int sms = aq_sm_count(cache->device);
+  if (P == 64) launch_rows_k<64>(a, cache->k_bits, cache->v_bits, append, sms, s);
+  else if (P == 128) launch_rows_k<128>(a, cache->k_bits, cache->v_bits, append, sms, s);
+  else launch_rows_k<256>(a, cache->k_bits, cache->v_bits, append, sms, s);
   return launched(fn) ? 0 : -1;
 }
 
@@ -177,7 +178,7 @@ int adaptq_rotary_apply(const adaptq_rotary_t *rotary, const void *x, int64_t x_
   // Several tokens a block where there are enough of them: all its threads form turns (16384 tokens x 32 heads x 128,
   // bf16: 46.4 us with four, 50.1 with one; few tokens would leave SMs idle).
   a.tokens_per_block = 1;
-  while (a.tokens_per_block < 4 && a.tokens_per_block * half < ROTARY_THREADS && n_tokens / (2 * a.tokens_per_block) >= 148 * 8) a.tokens_per_block *= 2;
+  while (a.tokens_per_block < 4 && a.tokens_per_block * half < ROTARY_THREADS && n_tokens / (2 * a.tokens_per_block) >= 8 * aq_sm_count(device)) a.tokens_per_block *= 2;
   const long long blocks = (n_tokens + a.tokens_per_block - 1) / a.tokens_per_block;
   if (blocks > 0x7fffffff) return fail(fn, "too many tokens for one call"), -1;
   a.heads_per_block = std::min(n_heads, (1 << 28) / dim); // all heads, as long as they are below 2^28 coordinates

@@ -7,18 +7,6 @@
 
 using namespace aq;
 
-// SMs of a device; what the workspace and the grid are sized for.
-static int sm_count(int device) {
-  static std::atomic<int> known[64] = {};
-  if (device < 0 || device >= 64) return 148;
-  int n = known[device].load();
-  if (!n) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return 148; }
-    known[device].store(n);
-  }
-  return n;
-}
-
 // The names below are the same in every unit: what differs between units carries the bit widths in its type.
 struct AttendRoom { size_t query_scales, block_headers, block_slots, warp_slots, warp_sums, total; }; // offsets in the workspace
 
@@ -37,7 +25,7 @@ template <typename S> static AttendRoom attend_room(int blocks, int cols, size_t
 template <typename S> static bool launch_attend(const AttendCall &call) {
   AttendLaunch &a = *call.launch;
   const char *fn = call.fn;
-  const int device = call.device, sms = sm_count(device);
+  const int device = call.device, sms = aq_sm_count(device);
   a.passes = (a.group + S::COLS - 1) / S::COLS;
   a.slot_cols = std::min(S::COLS, a.group);
   const long long items = (long long)a.n_seqs * a.c.heads * a.passes;
