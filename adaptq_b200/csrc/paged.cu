@@ -148,7 +148,13 @@ const attend_unit_t attend_units[3][3] = {{aq_attend_2_2, aq_attend_2_3, aq_atte
 int attend_mode(int type) { return type == TYPE_F32 ? ATTEND_EXACT : type == TYPE_F16 ? ATTEND_SPLIT : ATTEND_EIGHT; }
 
 // One exchange, so that a bit set by a call on another stream is either taken or left for the next time.
-__global__ void take_status_kernel(int *status, int *taken) { *taken = atomicExch(status, 0); }
+__global__ void take_status_kernel(int *status, int *taken) {
+  int bits = atomicExch(status, 0);
+#ifdef ADAPTQ_CHECKED
+  bits |= atomicExch(&rotary_status, 0);
+#endif
+  *taken = bits;
+}
 
 } // namespace
 

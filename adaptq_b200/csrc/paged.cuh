@@ -8,7 +8,15 @@
 namespace aq {
 
 enum { TYPE_F32 = 0, TYPE_F16 = 1, TYPE_BF16 = 2 };
-enum { PAGED_BAD_PAGE = 1, PAGED_BAD_POSITION = 2 };
+enum { PAGED_BAD_PAGE = 1, PAGED_BAD_POSITION = 2, PAGED_BAD_INDEX = 256 };
+
+// Checked build: an index check in front of an access, which is skipped if it fails, as AQ_CHECK; it leaves a bit in
+// the pool's status word.  The constant `true` otherwise.
+#ifdef ADAPTQ_CHECKED
+#define PAGED_CHECK(status_ptr, cond) ((cond) ? true : (atomicOr((status_ptr), PAGED_BAD_INDEX), false))
+#else
+#define PAGED_CHECK(status_ptr, cond) (true)
+#endif
 
 struct PagedView {
   uint8_t *k_pages, *v_pages;
@@ -102,6 +110,11 @@ template <typename F> __device__ __forceinline__ void with_type(int type, F f) {
   if (type == TYPE_BF16) f(TypeConstant<TYPE_BF16>());
   else if (type == TYPE_F16) f(TypeConstant<TYPE_F16>());
   else f(TypeConstant<TYPE_F32>());
+}
+
+// Rows of a side of the pool; `n` rows from `row` on lie in it.
+__device__ __forceinline__ bool rows_exist(const PagedView &c, long long row, int n) {
+  return row >= 0 && row + n <= (c.n_pages * c.heads) << c.page_shift;
 }
 
 // Page and place of position `pos` of a sequence whose table row is `row`; false (and a bit

@@ -49,6 +49,7 @@ template <typename S> static bool launch_attend(const AttendCall &call) {
   a.block_slots = reinterpret_cast<float *>(base + room.block_slots);
   a.warp_slots = reinterpret_cast<float *>(base + room.warp_slots);
   a.warp_sums = reinterpret_cast<float *>(base + room.warp_sums);
+  a.workspace_end = base + room.total;
   paged_query_kernel<S::DIM><<<(unsigned)items, QUERY_WARPS * 32, 0, call.stream>>>(
       a, S::COLS, 1.4426950408889634f / (S::DIM * table_scale(S::KEY_BITS)));
   if (!aq_launched(fn)) return false;

@@ -81,6 +81,11 @@ __device__ __forceinline__ int clipped_length(const AttendLaunch &a, int b, bool
   return n < 0 ? 0 : (int)room;
 }
 
+// n floats at p lie within the workspace (checked build).
+__device__ __forceinline__ bool in_workspace(const AttendLaunch &a, const void *p, size_t n) {
+  return p >= a.operands && static_cast<const float *>(p) + n <= a.workspace_end;
+}
+
 __device__ __forceinline__ int slot_floats(int cols, int P) { return cols * (P + 4); }
 
 // The factor by which the tables' values are larger than the codebook's: of all factors from 1 to 2, the one
@@ -150,6 +155,7 @@ template <int P> __device__ __forceinline__ void store_column(const AttendLaunch
   constexpr int E = P / 32;
   warp_butterflies<E>(v, lane);
   const float inv = sum == 0.f ? 0.f : 1.f / (sum * P);
+  if (!PAGED_CHECK(a.c.status, b >= 0 && b < a.n_seqs && h >= 0 && h < a.c.heads && query >= 0 && query < a.group)) return;
   const uint32_t signs = a.c.signs[h * E + lane / (32 / E)] >> (lane * E & 31);
   const long long at = (long long)b * a.out_seq + (long long)(h * a.group + query) * a.out_head + lane * E;
 #pragma unroll
@@ -196,6 +202,7 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
   }
 
   __device__ __forceinline__ void load_queries(const AttendLaunch &a, size_t item) {
+    if (!PAGED_CHECK(a.c.status, item < (size_t)a.n_seqs * a.c.heads * a.passes)) item = 0;
 #pragma unroll
     for (int i = 0; i < P / 8; ++i) qb[i] = a.operands[(item * (P / 8) + i) * 32 + lane];
 #pragma unroll
@@ -497,7 +504,7 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
         for (int i = 0; i < E; ++i) v[i] = (scratch[k * P + lane * E + i] + (SPLIT ? scratch[(k + 2) * P + lane * E + i] : 0.f)) * (1.f / table_scale(VB));
         const int col = 2 * k + e;
         if (whole) store_column<P>(a, b, h, pass * S::COLS + col, lane, v, sum);
-        else {
+        else if (PAGED_CHECK(a.c.status, col < a.slot_cols && in_workspace(a, slot, slot_floats(a.slot_cols, P)))) {
 #pragma unroll
           for (int i = 0; i < E; ++i) slot[col * P + lane * E + i] = v[i];
           if (lane == 0) *reinterpret_cast<float2 *>(slot + a.slot_cols * P + 2 * col) = make_float2(top, sum);
@@ -590,6 +597,7 @@ template <int P> __global__ void __launch_bounds__(QUERY_WARPS * 32) paged_query
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
       const int d = lane * E + i;
+      if (!PAGED_CHECK(a.c.status, (size_t)item < (size_t)a.n_seqs * per_seq && col < cols)) continue;
       uint32_t *to = a.operands + ((size_t)item * (P / 8) + (d % (P / 4)) / 2) * 32 + 4 * col + d / (P / 4);
       const uint32_t upper = pack2(v[i], v[i + 1], TYPE_F16);
       *to = upper;
@@ -660,7 +668,7 @@ template <typename S> struct AttendWalk {
   }
   __device__ __forceinline__ void find_pages(const AttendLaunch &a) {
     page = 0;
-    if (lane << a.c.page_shift < min(U, len - u * U))
+    if (lane << a.c.page_shift < min(U, len - u * U) && PAGED_CHECK(a.c.status, b >= 0 && b < a.n_seqs && u >= 0 && ((u * U) >> a.c.page_shift) + lane < a.table.width))
       page = a.table.entries[(long long)b * a.table.stride + ((u * U) >> a.c.page_shift) + lane];
   }
   // Start the copies of the next unit into `stage` and describe it; then, if there are more, find the one behind it.
@@ -678,6 +686,7 @@ template <typename S> struct AttendWalk {
       if (a.c.page_size >= U) {
         const long long row = (((long long)__shfl_sync(0xffffffffu, page, 0) * a.c.heads + h) << a.c.page_shift) + (tok0 & (a.c.page_size - 1));
         const uint8_t *k = a.c.k_pages + row * S::K_ROW + lane * 16, *v = a.c.v_pages + row * S::V_ROW + lane * 16;
+        if (!PAGED_CHECK(a.c.status, h >= 0 && h < a.c.heads && rows_exist(a.c, row, U))) return;
 #pragma unroll
         for (int i = 0; i < U * S::K_ROW / 512; ++i) copy_16(to + i * 512, k + i * 512);
 #pragma unroll
@@ -690,6 +699,7 @@ template <typename S> struct AttendWalk {
           const int per = a.c.page_size, at = p << a.c.page_shift;
           const long long row = ((long long)__shfl_sync(0xffffffffu, page, p) * a.c.heads + h) << a.c.page_shift;
           const uint8_t *k = a.c.k_pages + row * S::K_ROW, *v = a.c.v_pages + row * S::V_ROW;
+          if (!PAGED_CHECK(a.c.status, h >= 0 && h < a.c.heads && at + per <= U && rows_exist(a.c, row, per))) continue;
 #pragma unroll 1
           for (int i = lane * 16; i < per * S::K_ROW; i += 512) copy_16(to + at * S::K_ROW + i - lane * 16, k + i);
 #pragma unroll 1
@@ -752,8 +762,11 @@ __global__ void __launch_bounds__(AttendShape<KB, VB, P, MODE>::THREADS, 1) page
     const bool ends = d.z & 0x40000000;
     const bool stops = ends || i + 1 == units;
     if (__builtin_expect(!S::EXACT && !stops && d.z % w.KEEP == w.KEEP - 1, 0)) {
-      w.hand_over(a.warp_sums + (size_t)(blockIdx.x * S::WARPS + warp) * S::SUMS, handed);
-      handed = true;
+      float *place = a.warp_sums + (size_t)(blockIdx.x * S::WARPS + warp) * S::SUMS;
+      if (PAGED_CHECK(a.c.status, in_workspace(a, place, S::SUMS))) {
+        w.hand_over(place, handed);
+        handed = true;
+      }
     } else if (stops) {
       if (!S::EXACT && handed) w.take_back(a.warp_sums + (size_t)(blockIdx.x * S::WARPS + warp) * S::SUMS);
       const bool whole = ends && from_start;
@@ -790,7 +803,7 @@ __global__ void __launch_bounds__(AttendShape<KB, VB, P, MODE>::THREADS, 1) page
     }
     if (open >= 0 && chains[open].kind == 2) { bflags |= SEG_OPEN; bitem1 = chains[open].item; }
     *n_chains = n;
-    a.block_headers[blockIdx.x] = make_int4(bflags, bitem0, bitem1, 0);
+    if (PAGED_CHECK(a.c.status, n <= S::WARPS + 1 && in_workspace(a, a.block_headers + blockIdx.x, 4))) a.block_headers[blockIdx.x] = make_int4(bflags, bitem0, bitem1, 0);
   }
   __syncthreads();
   const int n = *n_chains, sf = slot_floats(a.slot_cols, P);
@@ -816,6 +829,7 @@ __global__ void __launch_bounds__(AttendShape<KB, VB, P, MODE>::THREADS, 1) page
     if (ch.kind == 0) store_column<P>(a, b, h, (hp - h * a.passes) * S::COLS + col, lane, v, L);
     else {
       float *to = a.block_slots + (size_t)(2 * blockIdx.x + ch.kind - 1) * sf;
+      if (!PAGED_CHECK(a.c.status, in_workspace(a, to, sf) && to + sf <= a.warp_slots)) continue;
 #pragma unroll
       for (int i = 0; i < P / 32; ++i) to[col * P + lane * (P / 32) + i] = v[i];
       if (lane == 0) *reinterpret_cast<float2 *>(to + a.slot_cols * P + 2 * col) = make_float2(M, L);
@@ -847,6 +861,7 @@ template <int P> __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_k
   const int sf = slot_floats(a.slot_cols, P);
   const int pieces = last - j + 1;
   auto piece = [&](int i) { return a.block_slots + (size_t)(2 * (j + i) + (i == 0)) * sf; };
+  if (!PAGED_CHECK(a.c.status, last < blocks && mine.z >= 0 && mine.z < a.n_seqs * a.c.heads * a.passes)) return;
   constexpr int E = P / 32;
   float v[E], M, L;
   join_pieces<P>(piece, pieces, warp, JOIN_WARPS, a.slot_cols, col, lane, v, M, L);

@@ -22,6 +22,7 @@ struct AttendLaunch {
   float *query_scales; // [item][8]
   int4 *block_headers;
   float *block_slots, *warp_slots, *warp_sums;
+  const void *workspace_end; // for the checked build
   int slot_cols; // columns of a partial result
 };
 

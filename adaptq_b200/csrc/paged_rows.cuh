@@ -167,6 +167,7 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
     const int row = min(r0 + lane / LANES, n_rows - 1), dt = row / heads, h = row - dt * heads;
     const int first_token = r0 / heads, nt = min(r0 + ROWS - 1, n_rows - 1) / heads - first_token + 1;
     const long long at = (t0 + dt) * src_token + h * src_head;
+    const bool row_exists = PAGED_CHECK(a.c.status, row >= 0 && t0 + dt < a.n_tokens && h < heads && first_token + nt <= tokens && d0 < P);
 
     float2 x[16];
 #pragma unroll
@@ -174,7 +175,7 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
     if (vec) with_type(a.type, [&](auto type) {
 #pragma unroll
       for (int i = 0; i < 32; i += 8)
-        if (d0 + i < dim) {
+        if (row_exists && d0 + i < dim) {
           float v[8];
           load_eight<decltype(type)::value>(src, at + d0 + i, v);
 #pragma unroll
@@ -183,8 +184,8 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
     }); else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        if (d0 + 2 * i < dim) x[i].x = load_one(src, at + d0 + 2 * i, a.type);
-        if (d0 + 2 * i + 1 < dim) x[i].y = load_one(src, at + d0 + 2 * i + 1, a.type);
+        if (row_exists && d0 + 2 * i < dim) x[i].x = load_one(src, at + d0 + 2 * i, a.type);
+        if (row_exists && d0 + 2 * i + 1 < dim) x[i].y = load_one(src, at + d0 + 2 * i + 1, a.type);
       }
     }
     const uint32_t signs = a.c.signs[h * LANES + part];
@@ -196,6 +197,7 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
         const long long pos = __shfl_sync(0xffffffffu, mine.pos, first_token + i);
         for (int pair = lane; pair < half; pair += 32) {
           const float2 k = rotary_turn(a.r, pair, pos);
+          if (!PAGED_CHECK(a.c.status, i < a.turn_tokens)) continue;
           turns[i * 2 * half + pair] = k.x;
           turns[i * 2 * half + half + pair] = k.y;
         }
@@ -265,6 +267,7 @@ __device__ __forceinline__ void append_rows(const RowsLaunch &a, const void *src
 
     if (r0 + lane / LANES < n_rows && page >= 0) {
       const long long slot = (((long long)page * heads + h) << a.c.page_shift) + off;
+      if (!PAGED_CHECK(a.c.status, rows_exist(a.c, slot, 1) && off >= 0 && off < a.c.page_size)) continue;
       store_words<BITS>(pages + slot * (P * BITS / 8) + part * (4 * BITS), w);
       if (part == 0) scales[slot] = norm;
     }
@@ -343,6 +346,7 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
       const int row = 16 * tile + g + 8 * r;
       if (row < nt && place[row].page >= 0) {
         const long long slot = (((long long)place[row].page * heads + h) << a.c.page_shift) + place[row].off;
+        if (!PAGED_CHECK(a.c.status, row < READ_TOKENS && h < heads && rows_exist(a.c, slot, 1))) continue;
         load_packed<N * BITS / 8>(pages + slot * (P * BITS / 8) + t * (N * BITS / 8), next[r]);
         norm[r] = scales[slot];
       }
@@ -412,7 +416,7 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
 #pragma unroll 1
         for (int i = 0; i < 8; ++i) {
           const int row = 16 * tile + 8 * r + i;
-          if (row >= nt || place[row].page < 0) continue;
+          if (row >= nt || place[row].page < 0 || !PAGED_CHECK(a.c.status, t0 + row < a.n_tokens && h < heads)) continue;
           uint16_t *to = static_cast<uint16_t *>(dst) + (t0 + row) * dst_token + h * dst_head;
           const uint16_t *from = reinterpret_cast<const uint16_t *>(stage + i * 4 * stage_part<P>);
 #pragma unroll 1
@@ -424,7 +428,7 @@ __device__ __forceinline__ void read_rows(const RowsLaunch &a, void *dst, long l
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = 16 * tile + g + 8 * r;
-      if (row >= nt || place[row].page < 0) continue;
+      if (row >= nt || place[row].page < 0 || !PAGED_CHECK(a.c.status, t0 + row < a.n_tokens && h < heads)) continue;
       const long long at = (t0 + row) * dst_token + h * dst_head + t * N;
       if (vec) with_type(a.type, [&](auto type) {
         constexpr int TYPE = decltype(type)::value;

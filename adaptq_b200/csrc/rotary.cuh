@@ -21,6 +21,10 @@ struct RotaryLaunch {
 
 constexpr int ROTARY_THREADS = 256;
 
+#ifdef ADAPTQ_CHECKED
+__device__ int rotary_status; // this kernel has no pool: adaptq_paged_take_status() adds its failed checks to the next one's
+#endif
+
 __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaunch a) {
   extern __shared__ float2 rotary_turns[]; // [tokens_per_block][r.dim / 2]
   const int half = a.r.dim >> 1;
@@ -33,7 +37,7 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
                                          : (long long)static_cast<const int *>(a.positions)[t0 + t];
     float2 cs = rotary_turn(a.r, pair, pos);
     if (a.inverse) cs.y = -cs.y;
-    rotary_turns[i] = cs;
+    if (PAGED_CHECK(&rotary_status, i >= 0 && i < a.tokens_per_block * half)) rotary_turns[i] = cs;
   }
   __syncthreads();
   if (a.vec) with_type(a.type, [&](auto type) {
@@ -44,6 +48,8 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
     for (int i = threadIdx.x; i < n; i += ROTARY_THREADS) {
       const int part = i % parts, th = i / parts, h = h0 + th % heads, t = th / heads;
       const long long xi = (t0 + t) * a.x_token + h * a.x_head, yi = (t0 + t) * a.y_token + h * a.y_head;
+      // the eights of this thread: at 8 part, behind `half` from there in the half layout
+      if (!PAGED_CHECK(&rotary_status, part >= 0 && h >= 0 && h < a.heads && t >= 0 && t < nt && 8 * part + (a.r.interleaved ? 8 : half + 8) <= a.dim)) continue;
       const float2 *cs = rotary_turns + t * half;
       float u[8], w[8];
       if (a.r.interleaved) {
@@ -82,6 +88,7 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryLaun
     for (int i = threadIdx.x; i < n; i += ROTARY_THREADS) {
       const int part = i % parts, th = i / parts, h = h0 + th % heads, t = th / heads;
       const long long xi = (t0 + t) * a.x_token + h * a.x_head, yi = (t0 + t) * a.y_token + h * a.y_head;
+      if (!PAGED_CHECK(&rotary_status, part >= 0 && h >= 0 && h < a.heads && t >= 0 && t < nt && half + part < a.dim)) continue;
       if (part < half) {
         const int d = a.r.interleaved ? 2 * part : part, e = a.r.interleaved ? d + 1 : d + half;
         const float2 k = rotary_turns[t * half + part];

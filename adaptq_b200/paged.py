@@ -17,7 +17,8 @@ import torch
 from . import _lib
 from .rotary import TYPES, Rotary, check_written, current_stream, increment_version
 
-_STATUS = ((1, "a block table names a page outside the pool"), (2, "a position or length has no room in its block table"))
+_STATUS = ((1, "a block table names a page outside the pool"), (2, "a position or length has no room in its block table"),
+           (256, "a device-side index check failed (checked build), the access was skipped"))
 
 
 def _padded(dim: int) -> int:

@@ -16,7 +16,8 @@
  *
  * Values that only the device knows are checked there: an entry that would leave the
  * pool or the table is skipped and leaves a bit in *status -- 1: a page number outside the
- * pool, 2: a position or length that the block table has no room for.  The caller zeroes the
+ * pool, 2: a position or length that the block table has no room for, 256: an index check of the
+ * checked build failed.  The caller zeroes the
  * word at first; adaptq_paged_take_status() reads and zeroes it in one step, beside whatever
  * calls are under way.
  */
