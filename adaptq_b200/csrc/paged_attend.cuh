@@ -53,7 +53,7 @@ template <int KB, int VB, int P, int MODE> struct AttendShape {
   static constexpr int K_ROW = P * KB / 8, V_ROW = P * VB / 8;
   static constexpr int STAGE = U * (K_ROW + V_ROW + 8);
   static constexpr int COLS = SPLIT ? 4 : 8; // queries of a pass
-  static constexpr int SUMS = EXACT ? 0 : 8 * P + 64; // floats of the workspace for the sums of a warp under way
+  static constexpr int SUMS = 8 * P + 128; // floats of the workspace for the sums of a warp under way
   static constexpr int table_bytes(int bits) { return bits == 2 && !EXACT ? 32768 : 128 << (2 * bits); }
   static constexpr int K_TABLE = 0, V_TABLE = KB == VB ? 0 : table_bytes(KB);
   static constexpr int TABLES = table_bytes(KB) + (KB == VB ? 0 : table_bytes(VB));
@@ -437,22 +437,26 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
     }
   }
 
-  // The tensor cores cut sums off instead of rounding them, 2^-23 of the sum a product, all to one side.  So a long run
-  // hands its sums over every KEEP units: to `place` (a lane's own words in the workspace, with the references they are
-  // relative to), which is added up in float32 and comes back at the end (131072 tokens of one direction a warp: 9e-4
-  // of the sum before, 2e-5 now; 64 x 8 heads x 8192 tokens: 78.4 us before, 79.2 now, through the registers that the code
-  // takes).  EXACT does not need it.
+  // The tensor cores cut sums off instead of rounding them, 2^-23 of the sum a product, all to one side, and a float32 sum
+  // that holds one large term loses what is added to it in small pieces.  So a long run hands its sums over every KEEP
+  // units: to `place` (a lane's own words in the workspace, with the references they are relative to), which is added up
+  // in float32 and comes back at the end.  131072 tokens of one direction a warp: 9e-4 of the sum before, 2e-5 now; as
+  // many of 2^-27 of one before them, float32: 2e-4, 7e-6 now; 64 x 8 heads x 8192 tokens: 78.4 us, 79.2 now, through the
+  // registers that the code takes.
   static constexpr int KEEP = 64;
   __device__ __forceinline__ void hand_over(float *place, bool more) {
     float4 *mine = reinterpret_cast<float4 *>(place) + lane;
-    float2 *refs = reinterpret_cast<float2 *>(place + 8 * P) + lane;
+    float4 *sums = reinterpret_cast<float4 *>(place + 8 * P) + lane; // references and sums of weights
     float ratio[2] = {0.f, 0.f};
     if (more) {
-      const float2 old = *refs;
+      const float4 old = *sums;
       ratio[0] = exp2_approx(old.x - ref[0]);
       ratio[1] = exp2_approx(old.y - ref[1]);
+      l[0] = fmaf(old.z, ratio[0], l[0]);
+      l[1] = fmaf(old.w, ratio[1], l[1]);
     }
-    *refs = make_float2(ref[0], ref[1]);
+    *sums = make_float4(ref[0], ref[1], l[0], l[1]);
+    l[0] = l[1] = 0.f;
 #pragma unroll
     for (int j = 0; j < DIM_TILES; ++j) {
       const float4 old = more ? mine[32 * j] : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -463,8 +467,10 @@ template <int KB, int VB, int P, int MODE> struct AttendWarp {
   }
   __device__ __forceinline__ void take_back(const float *place) {
     const float4 *mine = reinterpret_cast<const float4 *>(place) + lane;
-    const float2 old = reinterpret_cast<const float2 *>(place + 8 * P)[lane];
+    const float4 old = reinterpret_cast<const float4 *>(place + 8 * P)[lane];
     const float ratio[2] = {exp2_approx(old.x - ref[0]), exp2_approx(old.y - ref[1])};
+    l[0] = fmaf(old.z, ratio[0], l[0]);
+    l[1] = fmaf(old.w, ratio[1], l[1]);
 #pragma unroll
     for (int j = 0; j < DIM_TILES; ++j) {
       const float4 v = mine[32 * j];
@@ -761,14 +767,14 @@ __global__ void __launch_bounds__(AttendShape<KB, VB, P, MODE>::THREADS, 1) page
     if (d.w > 0) w.unit(stage, d.w);
     const bool ends = d.z & 0x40000000;
     const bool stops = ends || i + 1 == units;
-    if (__builtin_expect(!S::EXACT && !stops && d.z % w.KEEP == w.KEEP - 1, 0)) {
+    if (__builtin_expect(!stops && d.z % w.KEEP == w.KEEP - 1, 0)) {
       float *place = a.warp_sums + (size_t)(blockIdx.x * S::WARPS + warp) * S::SUMS;
       if (PAGED_CHECK(a.c.status, in_workspace(a, place, S::SUMS))) {
         w.hand_over(place, handed);
         handed = true;
       }
     } else if (stops) {
-      if (!S::EXACT && handed) w.take_back(a.warp_sums + (size_t)(blockIdx.x * S::WARPS + warp) * S::SUMS);
+      if (handed) w.take_back(a.warp_sums + (size_t)(blockIdx.x * S::WARPS + warp) * S::SUMS);
       const bool whole = ends && from_start;
       const int slot = from_start ? 1 : 0;
       w.finish(a, d.x, h, pass, min(S::COLS, a.group - pass * S::COLS), whole, slots + slot * slot_floats(a.slot_cols, P),

@@ -134,3 +134,55 @@ def test_coordinates_at_a_threshold(gen, bits):
         code = ref.unpack(pages[0, 0, :n], bits).cpu()
         expect = torch.tensor(want)
         assert torch.equal(code[:, ::2], expect[:, :1].expand(n, 32)) and torch.equal(code[:, 1::2], expect[:, 1:].expand(n, 32))
+
+
+@pytest.mark.parametrize("dtype,power,tolerance", [(F32, 27, 2e-5), (F32, 30, 2e-5), (F16, 24, 3.8e-3), (BF16, 22, 1.06e-2)])
+def test_many_tokens_far_below_one_in_a_warp(gen, dtype, power, tolerance):
+    """One value 2^power times as long as 131071 others of its sequence under equal weights, thousands of whose units
+    one warp holds together with it: without them the output would be off by 131071 / 2^power, which is above what is
+    tolerated."""
+    seqs, n, page = 148 * 16, 131072, 256
+    assert (n - 1) * 2.0 ** -power > 2 * tolerance
+    cache, signs = make_cache(gen, n // page, 1, 128, 4, 4, page)
+    ref.random_pool(cache, gen)
+    cache.k_scales.zero_()                                   # equal logits
+    cache.v_pages[:] = cache.v_pages[0, 0, 0]                # one row for all but one
+    cache.v_scales.fill_(1.375)
+    order = torch.randperm(n // page, generator=gen, device="cuda").int()
+    for unit in (0, 300, 511):
+        cache.v_pages[:] = cache.v_pages[int(order[100]), 0, 0]
+        cache.v_scales.fill_(1.375)
+        page_of = int(order[unit])
+        cache.v_scales[page_of, 0, 11] = 1.375 * 2.0 ** power
+        cache.v_pages[page_of, 0, 11] = cache.v_pages[page_of, 0, 11].flip(0)   # another direction
+        q = torch.randn(1, 1, 128, generator=gen, device="cuda").to(dtype)
+        want = ref.attend(cache, signs, q, order[None], ints(n))
+        got = cache.attend(q.expand(seqs, -1, -1), order[None].expand(seqs, -1), torch.full((seqs,), n, dtype=torch.int32, device="cuda"))
+        attend_close(got, want.expand(seqs, -1, -1), dtype, f"page {unit}")
+
+
+@pytest.mark.parametrize("where", [0, 300, 511])
+def test_many_weights_far_below_one_in_a_warp(gen, where):
+    """As above in float32 with one weight of 2^27 among equal ones, so that the sum of weights is what would lose
+    them.  Their share is 131071 / 2^27 = 9.8e-4.  Logits reach 40 and are off by 2^-20 of one (10 roundings of 2^-23
+    each), weights as much of themselves."""
+    seqs, n, page, power, dim = 148 * 16, 131072, 256, 27, 128
+    cache, signs = make_cache(gen, n // page, 1, dim, 4, 4, page)
+    ref.random_pool(cache, gen)
+    for t in (cache.k_pages, cache.v_pages):
+        t[:] = t[0, 0, 0].clone()
+    cache.k_scales.fill_(1.0)
+    cache.v_scales.fill_(1.375)
+    order = torch.randperm(n // page, generator=gen, device="cuda").int()
+    q = torch.randn(1, 1, dim, generator=gen, device="cuda")
+    _, level, _ = ref.rows(cache, "k", order[:1].long(), torch.zeros(1, dtype=torch.long, device="cuda"), signs)
+    z = (q.double() * signs) @ ref.hadamard(dim).cuda()
+    q *= float(10.0 / ((z * level).sum() * dim ** -0.5 / dim))   # a logit of 10 where the norm is one
+    cache.k_scales[int(order[where]), 0, 11] = 1.0 + power * math.log(2.0) / 10.0
+    cache.v_pages[int(order[where]), 0, 11] = cache.v_pages[int(order[where]), 0, 11].flip(0)   # another direction
+    want = ref.attend(cache, signs, q, order[None], ints(n))
+    got = cache.attend(q.expand(seqs, -1, -1), order[None].expand(seqs, -1), torch.full((seqs,), n, dtype=torch.int32, device="cuda"))
+    share = 131071 / (131071 + 2.0 ** power)
+    alone = ref.attend(cache, signs, q, order[None, where: where + 1], ints(12))   # the one and eleven others: without the rest
+    assert float((alone - want).norm() / want.norm()) > 20 * 2e-5 and share > 20 * 2e-5
+    attend_close(got, want.expand(seqs, -1, -1), F32)
