@@ -186,3 +186,71 @@ def test_many_weights_far_below_one_in_a_warp(gen, where):
     alone = ref.attend(cache, signs, q, order[None, where: where + 1], ints(12))   # the one and eleven others: without the rest
     assert float((alone - want).norm() / want.norm()) > 20 * 2e-5 and share > 20 * 2e-5
     attend_close(got, want.expand(seqs, -1, -1), F32)
+
+
+def evaluate(cache, signs, q, table, lengths, queries=lambda z: z, weights=lambda w: w, level=lambda c: c):
+    """The attention in 64 bits with roundings planted: of the transformed queries, of weights times norms (relative to the
+    largest), of the codebook."""
+    p, dim, heads = signs.shape[1], cache.dim, cache.n_kv_heads
+    out, group, h = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), q.shape[1] // heads, ref.hadamard(p).cuda()
+    for b, n in enumerate(lengths):
+        at, off = ref.place(cache, table[b], n)
+        _, kl, kn = ref.rows(cache, "k", at, off, signs)
+        _, vl, vn = ref.rows(cache, "v", at, off, signs)
+        full = torch.zeros(heads, group, p, dtype=torch.float64, device="cuda")
+        full[..., :dim] = q[b].double().view(heads, group, dim)
+        z = queries((full * signs[:, None]) @ h)
+        logit = torch.einsum("hgp,thp->hgt", z, level(kl)) * kn.T[:, None] * dim ** -0.5 / p
+        w = torch.softmax(logit, -1)
+        out[b] = (torch.einsum("hgt,thp->hgp", weights(w * vn.T[:, None]), level(vl)) @ h * signs[:, None] / p)[..., :dim].reshape(-1, dim)
+    return out
+
+
+LONG, SHORT = [600, 64, 1000, 333, 777, 150], [2 + b % 7 for b in range(24)]
+
+
+@pytest.mark.parametrize("dtype,kb,vb,lengths", [(F16, 4, 4, LONG), (F16, 3, 2, LONG), (F16, 2, 3, LONG), (F16, 3, 2, SHORT), (F16, 2, 3, SHORT),
+                                                 (BF16, 4, 4, LONG), (BF16, 3, 2, LONG)])
+def test_precision_of_16_bit_calls(gen, dtype, kb, vb, lengths):
+    """Error of float16 and bfloat16 calls against what their arithmetic is said to leave.
+
+    float16: queries and weights have 22 bits; the codebook is off by c = 7.8e-5 (4 bits), 2.7e-6 (3) or 1.7e-8 (2) of a value,
+    rms over its use.  Terms add up at random, so logits of spread s move weights by c_k s and values move by c_v, and
+    the sums in float32 add 2e-6: eta = sqrt((c_k s)^2 + c_v^2) + 2e-6 of the output.  bfloat16: queries, weights and values
+    have 11 bits, 2^-12 rms at most: eta = sqrt(2) 2^-12 sqrt(s^2 + 1).
+    Independent of that is rho, the output's own rounding, which the definition tells.  So the norm of the error over all
+    outputs is at most sqrt(rho^2 + eta^2), and 5 % for the sample.  A float16 output differs from the rounded definition
+    where a border between two roundings, at least 2^-11 |y| apart, lies within the error: a share of at most
+    min(1, 2^11 eta Y / |y|), where Y is the rms of its head's outputs.
+    The same evaluation with one rounding more, planted in the definition, lies above that."""
+    seqs, heads, group, dim = len(lengths), 4, 4, 128
+    cache, signs = make_cache(gen, 120, heads, dim, kb, vb, 64)
+    ref.random_pool(cache, gen)
+    table = ref.random_table(cache, lengths, gen)
+    q = (1.5 * torch.randn(seqs, heads * group, dim, generator=gen, device="cuda")).to(dtype)
+    want = evaluate(cache, signs, q, table, lengths)
+    attend_close(want, ref.attend(cache, signs, q, table, ints(*lengths)), F32)
+    error = lambda y: float((y.double() - want).norm() / want.norm())  # noqa: E731
+    other = lambda y: float((y != want.to(dtype)).double().mean())  # noqa: E731
+    rho, spread = error(want.to(dtype)), 1.5 * 1.1   # norms vary by a third around sqrt(dim), which adds a tenth
+    if dtype == F16:
+        c = {4: 7.8e-5, 3: 2.7e-6, 2: 1.7e-8}
+        eta = math.hypot(c[kb] * spread, c[vb]) + 2e-6
+    else:
+        eta = math.sqrt(2) * 2.0 ** -12 * math.hypot(spread, 1.0)
+    bound = 1.05 * math.hypot(rho, eta)
+    share = float((2.0 ** 11 * eta * want.pow(2).mean(-1, keepdim=True).sqrt() / want.abs()).clamp(max=1).mean())
+    got = cache.attend(q, table, ints(*lengths))
+    assert error(got) <= bound, f"{error(got):.3e} > {bound:.3e} (rounding alone {rho:.3e})"
+    if dtype != F16:
+        return
+    assert other(got) <= share, f"{other(got):.4f} of the outputs are rounded otherwise, {share:.4f} may be"
+    # one part of float16 for queries or weights (the largest of them 400, some number that is not a power of two), or the
+    # codebook as float16 holds it
+    half = lambda x: (x * (400 / x.abs().amax(-1, keepdim=True))).half().double() * (x.abs().amax(-1, keepdim=True) / 400)  # noqa: E731
+    planted = evaluate(cache, signs, q, table, lengths, weights=half).to(dtype)
+    assert error(planted) > bound or other(planted) > share or kb == vb == 4
+    planted = evaluate(cache, signs, q, table, lengths, queries=half).to(dtype)
+    assert error(planted) > bound
+    planted = evaluate(cache, signs, q, table, lengths, level=lambda x: x.half().double()).to(dtype)
+    assert error(planted) > bound
