@@ -1,9 +1,9 @@
-"""Calls of the paged cache and of Rotary next to other streams and to automatic differentiation."""
+"""Calls of the paged cache and of Rotary next to other streams, to automatic differentiation and to missing pages."""
 import pytest
 import torch
 
 import paged_reference as ref
-from test_gpu_paged import BF16, F32, SCALINGS, ints, make_cache
+from test_gpu_paged import BF16, E, F16, F32, SCALINGS, attend_close, close, ints, make_cache, rotary_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +149,57 @@ def test_refused_steps_store_nothing(gen):
         assert all(torch.equal(a, b) for a, b in zip(before, (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales)))
     cache.step(k, k, q, table, n)
     assert not torch.equal(before[0], cache.k_pages)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("interleaved,dim,part", [(False, 128, 128), (True, 80, 40), (False, 67, 30)])
+def test_rotary_gradient_in_16_bits(gen, dtype, interleaved, dim, part):
+    from adaptq_b200 import Rotary
+    r = Rotary(part, interleaved=interleaved, scaling=SCALINGS[3])
+    x = torch.randn(40, 3, dim, generator=gen, device="cuda").to(dtype).requires_grad_()
+    g = torch.randn(40, 3, dim, generator=gen, device="cuda").to(dtype)
+    pos = torch.randint(0, 2 ** 20, (40,), generator=gen, device="cuda")
+    (dx,) = torch.autograd.grad(r(x, pos), x, g)
+    want = ref.rotate(g.double(), pos, r, inverse=True)
+    b, tiny = rotary_bound(g.double(), pos, r, dtype)
+    assert dx.dtype == dtype
+    close(dx, want, b + E[dtype] * want.abs() + tiny)
+    # differences of a linear map are its values: <R s, g> = <s, R^T g>, up to the roundings of both to 16 bits
+    s = torch.randn(40, 3, dim, generator=gen, device="cuda").to(dtype)
+    left, right = (r(s, pos).double() * g.double()), (s.double() * dx.double())
+    room = E[dtype] * float(left.abs().sum() + right.abs().sum()) + 2 * 7e-7 * r.factor * 2 * float((s.double().abs() * g.double().abs().amax()).sum())
+    assert abs(float(left.sum() - right.sum())) <= room
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (256, 16), (128, 64), (64, 128)])
+def test_units_with_missing_pages_are_left_out(gen, dtype, dim, page):
+    """A page that does not exist takes the tokens of its unit along (64 of them, 32 above 128 coordinates; at pages
+    larger than that its own); what is left attends as if those tokens had not been there."""
+    unit = 32 if dim > 128 else 64
+    span = max(unit, page)
+    cache, signs = make_cache(gen, 5 * span // page + 2, 2, dim, 4, 3, page)
+    ref.random_pool(cache, gen)
+    n, per = 4 * span + 5, span // page
+    table = ref.random_table(cache, [n, 0], gen)
+    table[1] = table[0]
+    q = torch.randn(2, 6, dim, generator=gen, device="cuda").to(dtype)
+    whole = ref.attend(cache, signs, q, table, ints(n, n))
+    got = cache.attend(q, table, ints(n, n))
+    attend_close(got, whole, dtype)
+    cache.check()
+    for missing, value in ((1 * per, -1), (2 * per + per - 1, cache.n_pages), (0, 2 ** 31 - 1), (4 * per, -2 ** 31)):
+        broken = table.clone()
+        broken[0, missing] = value
+        got = cache.attend(q, broken, ints(n, n))
+        with pytest.raises(RuntimeError, match="outside the pool"):
+            cache.check()
+        u = missing // per                       # the span that is gone, the last one has five tokens
+        left = torch.cat([table[0, : u * per], table[0, (u + 1) * per:]])
+        m = n - (span if u < 4 else 5)
+        want = torch.cat([ref.attend(cache, signs, q[:1], left[None], ints(m)), whole[1:]])
+        attend_close(got, want, dtype, f"page {missing}")
+    got = cache.attend(q, torch.full_like(table, -1), ints(n, 0))
+    assert not bool(got.any())
+    with pytest.raises(RuntimeError, match="outside the pool"):
+        cache.check()
