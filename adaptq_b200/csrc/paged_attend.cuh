@@ -660,6 +660,7 @@ template <typename S> struct AttendWalk {
     const int at = 31 - __clz(__ballot_sync(0xffffffffu, before <= rest));
     rest -= __shfl_sync(0xffffffffu, before, at);
     for (b = at * chunk;; ++b) {
+      if (b >= a.n_seqs) { b = 0; return 0; } // lengths that someone changed meanwhile must not lead out of them
       len = clipped_length(a, b, false);
       nu = (len + U - 1) / U;
       if (rest < nu * per_seq) break;
@@ -721,7 +722,8 @@ template <typename S> struct AttendWalk {
         pass = 0;
         if (++h == a.c.heads) {
           h = 0;
-          do len = clipped_length(a, ++b, false); while (len == 0);
+          do len = ++b < a.n_seqs ? clipped_length(a, b, false) : 0; while (len == 0 && b < a.n_seqs);
+          b = min(b, a.n_seqs - 1); // see start()
           nu = (len + U - 1) / U;
         }
       }

@@ -203,3 +203,24 @@ def test_units_with_missing_pages_are_left_out(gen, dtype, dim, page):
     assert not bool(got.any())
     with pytest.raises(RuntimeError, match="outside the pool"):
         cache.check()
+
+
+def test_lengths_that_change_during_a_call(gen):
+    """A caller's mistake, whose outputs nobody can tell, but which must not lead a kernel out of its tensors."""
+    cache, signs = make_cache(gen, 400, 8, 128, 4, 2, 16)
+    ref.random_pool(cache, gen)
+    table = torch.randint(0, 400, (64, 100), generator=gen, device="cuda", dtype=torch.int32)
+    n, other = (torch.randint(0, 1601, (64,), generator=gen, device="cuda", dtype=torch.int32) for _ in range(2))
+    other[torch.rand(64, generator=gen, device="cuda") < 0.5] = 0
+    q = torch.randn(64, 16, 128, generator=gen, device="cuda").to(BF16)
+    lengths, side = n.clone(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(100):
+        with torch.cuda.stream(side):
+            for new in (other, torch.zeros_like(n), n, other.flip(0)):
+                lengths.copy_(new)
+        for _ in range(4):
+            cache.attend(q, table, lengths)
+    torch.cuda.synchronize()
+    cache.check()
+    attend_close(cache.attend(q, table, n), ref.attend(cache, signs, q, table, n), BF16)
