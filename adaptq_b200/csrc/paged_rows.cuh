@@ -3,9 +3,9 @@
 // Append: a row of P coordinates is held by P/32 lanes, 32 consecutive ones each, two in a
 // register pair (the float2 instructions round each half like the scalar ones): five of the
 // log2 P butterfly stages stay inside a lane, the others are shuffles, and a lane's codes are
-// a whole number of words.  Bound by instructions: 109 a row of 128 coordinates (rotation 28,
-// transform 22, quantiser 24 of those of a 4-bit key), 2.6 a clock; four prompts of 3277 to 8192
-// tokens x 8 heads in bf16 at K4/V2 take 62 us, 19 at the copy rate.
+// a whole number of words.  Bound by instructions: 117 a row of 128 coordinates (transform 22,
+// quantiser 24 of those of a 4-bit key), 2.6 a clock; four prompts of 3277 to 8192
+// tokens x 8 heads in bf16 at K4/V2 take 61 us, 19 at the copy rate.
 // Read-back: see paged_read_kernel.
 #pragma once
 #include "paged.cuh"
@@ -294,7 +294,7 @@ template <int P, int KB, int VB> __global__ void __launch_bounds__(ROWS_THREADS,
 // (g, t) holds the coordinates t*P/4 .. of the rows g and g+8; the eight of a step are {t*P/4 + 2s + i}, i < 2, so
 // the product transforms along t and i, and log2(P/8) stages of butterflies along s remain inside the lane.  22 bits
 // of the codebook and float32 sums: as exact as the butterflies alone, which cost a quarter more time.  Bound by
-// instructions (49 a row of 128, 2.2 a clock at 16 warps an SM): 30512 tokens x 8 heads at K4/V4 in fp16 take 46 us, 24 at
+// instructions (49 a row of 128, 2.2 a clock at 16 warps an SM): 30512 tokens x 8 heads at K4/V4 in fp16 take 44 us, 24 at
 // the copy rate.
 template <int BITS> __device__ __forceinline__ uint32_t code_bytes(const uint32_t *w, int i, const uint32_t *g24) {
   // a word that holds code i in its byte (see code_byte)

@@ -238,7 +238,7 @@ class PagedKVCache:
     def check(self):
         """Wait for the device -- all of its streams -- and raise RuntimeError if a call since the last check named a page
         outside the pool, or a position or length without room in its block table (those entries were skipped).  Calls that
-        other threads make meanwhile report here or at the next check."""
+        other threads make meanwhile report here or at the next check.  Not while a stream is being captured."""
         torch.cuda.synchronize(self.device)
         taken = torch.empty(1, dtype=torch.int32, device=self.device)
         if self._L.adaptq_paged_take_status(self._ref, taken.data_ptr(), current_stream(self._index)):

@@ -94,8 +94,9 @@ int adaptq_paged_read(const adaptq_paged_t *cache, void *k_out, int64_t k_token_
  * Logits are scale * q.k (scale > 0; the rings' is 1 / sqrt(dim)); queries are rotated by
  * position lengths[b] - 1 first, if `rotary`.  A sequence of length 0 gives zeros.  float32
  * calls are computed to float32's precision throughout (codebook, queries and weights in two
- * float16 parts); float16 calls hold queries and weights in two parts, bfloat16 calls in one;
- * sums are float32.  Tokens are taken 64 at a time (32 above 128 coordinates): one page that
+ * float16 parts); float16 calls hold queries and weights in two parts, bfloat16 calls in one,
+ * both the codebook in one (off by 1.0e-4 of a value at 4 bits, 3.7e-6 at 3, 1.7e-8 at 2);
+ * sums are float32, over at most 4096 tokens at a time.  Tokens are taken 64 at a time (32 above 128 coordinates): one page that
  * does not exist leaves all of its 64 out.
  * workspace: adaptq_paged_attend_workspace() bytes, 16-byte aligned, whose contents need not
  * be kept between calls; calls that may overlap need one each. */
