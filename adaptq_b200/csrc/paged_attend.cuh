@@ -25,8 +25,8 @@
 //            operations per word.
 // What bounds it: latency at the eight to twelve warps an SM that the rings leave room for.  The shared-memory pipe
 // is 0.7 busy over the call (380 wavefronts a unit of 64 tokens, 128 coordinates at K4/V2: 256 of look-ups, the rest
-// copies, rows and norms), the issue slots half, behind 6 us of set-up.  64 sequences of 820 to 8192 tokens x 8 KV heads x 4 queries: 79 us, 3.1 TB/s; one of 131072 tokens at
-// K4/V4: 50 us, 2.8 TB/s.
+// copies, rows and norms), the issue slots half, behind 6 us of set-up.  64 sequences of 820 to 8192 tokens x 8 KV heads
+// x 4 queries: 79 us, 3.1 TB/s; one of 131072 tokens at K4/V4: 50 us, 2.8 TB/s.
 // tcgen05 would take its operands from shared or tensor memory: the expanded rows (512 bytes a
 // token and head) would have to be stored first, 256 wavefronts a unit more for the pipe that is busiest here;
 // mma.sync takes them from the registers in which the look-up leaves them.
